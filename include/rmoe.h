@@ -49,7 +49,7 @@
 extern "C" {
 #endif
 
-#define RMOE_ABI_VERSION 6
+#define RMOE_ABI_VERSION 7
 
 #define RMOE_OK 0
 #define RMOE_EINVAL (-1) /* inconsistent or unsupported shape / argument */
@@ -335,6 +335,148 @@ int rmoe_dequantize(const rmoe_qweight* w, int64_t row_begin, int64_t rows,
  * bandwidth for a given launch shape. */
 int rmoe_stream_read(const void* buffer, size_t bytes, uint32_t* partials,
                      int32_t blocks, void* stream);
+
+/* ---- The decoder layer's other half: the token mixer (came with ABI
+ * version 7).  No counterpart in the reference, whose attention and linear
+ * attention are mlx-lm's; the layers are those of docs/architecture.md:31-37.
+ * The calls below keep no counters: their workspaces need no zero-fill and
+ * hold nothing between calls. */
+
+/* Rows of heads: value d of head h of row t is x[t * row_stride + h *
+ * head_stride + d], bf16; x 16-byte aligned, strides multiples of 8. */
+typedef struct rmoe_rows {
+  const uint16_t* x;
+  int64_t row_stride;
+  int64_t head_stride;
+  int32_t heads;
+} rmoe_rows;
+
+/* A paged key-value cache: value d of token i of page p and key head h is at
+ * p * page_stride + h * head_stride + i * row_stride + d of k and of v
+ * (values; 16-byte aligned bases, strides multiples of 16 bytes).  bits 16:
+ * bf16; bits 8: e4m3 (fn), a value being k_scale (v_scale) times its code.
+ * page_size a power of two, 8..1024; dim 64, 96, 128, 192 or 256. */
+typedef struct rmoe_paged_cache {
+  void* k;
+  void* v;
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t row_stride;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t dim;
+  int32_t bits;
+  float k_scale; /* read at bits 8 */
+  float v_scale;
+} rmoe_paged_cache;
+
+/* Which values of a head turn, and by which positions: the first 2 * half,
+ * pair i by position[axis(i)] * inv_freq[i] (inv_freq device fp32 [half]).
+ * Pair i is values (i, i + half), or (2 i, 2 i + 1) when `adjacent`.  axes
+ * 1..4 with sections[0..axes) summing to half: the pairs' axes one section
+ * after the other, or, when `woven`, axis i mod axes as long as that axis's
+ * section has pairs left (i / axes < section) and axis 0 beyond; a woven
+ * section of another axis may not exceed its turns.  half a multiple of 8,
+ * at most 128. */
+typedef struct rmoe_rotary_spec {
+  const float* inv_freq;
+  int32_t half;
+  int32_t axes;
+  int32_t sections[4];
+  int32_t woven;
+  int32_t adjacent;
+} rmoe_rotary_spec;
+
+/* One step's bookkeeping from lengths on the device.  cached / added int32
+ * [requests] (negative counts as 0; at most 4096 requests): tokens that
+ * request r holds, and tokens it takes in this step.  Its pages from entry
+ * ceil(cached / page_size) of block_table row r on, as many as cached +
+ * added tokens need and table_width has room for, come from free_pages
+ * [free_count] in order of request, then entry; past the end of that list
+ * the entry becomes -1.  Other entries are left as they were.
+ * Written: cu_seqlens [requests + 1], the running sum of added; lengths
+ * [requests] = cached + added; counts [3]: tokens, pages taken, pages that
+ * were missing (sums that pass INT32_MAX stay there); and for each of `rows`
+ * rows, the tokens of all requests one after the other: slots (page *
+ * page_size + place in it, or -1 where the token has no page), positions
+ * (cached + place among the request's new tokens) and request_of; rows
+ * behind the last token get -1, 0 and -1. */
+int rmoe_paged_tables(const int32_t* cached, const int32_t* added, int32_t requests,
+                      int32_t* block_table, int64_t table_stride, int32_t table_width,
+                      const int32_t* free_pages, int32_t free_count, int32_t page_size,
+                      int32_t rows, int64_t* slots, int32_t* positions, int32_t* request_of,
+                      int32_t* cu_seqlens, int32_t* lengths, int32_t* counts, void* stream);
+
+/* Rotary positions: q_out [rows, q heads, dim] and k_out [rows, k heads, dim]
+ * = the turned rows (angles in 64 bits, products fp32, one rounding), values
+ * past 2 * half copied.  positions int32, axis a's at positions + a *
+ * axis_stride.  dim a multiple of 8, at most 1024.  Outputs must not overlap
+ * inputs. */
+int rmoe_rotary(const rmoe_rotary_spec* spec, const int32_t* positions, int64_t axis_stride,
+                int32_t rows, int32_t dim, const rmoe_rows* q, uint16_t* q_out,
+                const rmoe_rows* k, uint16_t* k_out, void* stream);
+
+/* The same with the turned keys and the values v written into the cache:
+ * row t at slot slots[t] (int64, as rmoe_paged_tables gives them); a row whose
+ * slot is outside the cache's writes nothing there.  bits 8: e4m3 of x * fp32(1
+ * / scale), to nearest even, saturating.  Rows with one slot in common leave
+ * either's values. */
+int rmoe_rotary_append(const rmoe_rotary_spec* spec, const int32_t* positions,
+                       int64_t axis_stride, int32_t rows, const rmoe_rows* q, uint16_t* q_out,
+                       const rmoe_rows* k, const rmoe_rows* v, const rmoe_paged_cache* cache,
+                       const int64_t* slots, void* stream);
+
+/* Attention of one new token of each request over its cached keys:
+ * out [requests, q->heads, dim] = softmax_j(scale q.k_j) v_j over j <
+ * lengths[r], with window > 0 over the last `window` of them; query heads
+ * [h G, (h + 1) G) read key head h, G = q->heads / kv_heads.  block_table
+ * int32 [requests, table_width] (row stride table_stride); lengths past
+ * table_width * page_size end there.  Keys of a page outside [0, pages) do
+ * not count, whatever the cache holds.  A request without keys gets zeros and
+ * lse -inf.  lse fp32 [requests, q->heads] (natural logarithm of the sum of
+ * exp(scale q.k)) may be NULL.  The probabilities are rounded to bf16 for
+ * their product with v; all else is fp32.  workspace: at least
+ * rmoe_paged_attention_workspace_bytes, 16-byte aligned. */
+int rmoe_paged_attention(const rmoe_rows* q, const rmoe_paged_cache* cache,
+                         const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                         const int32_t* lengths, int32_t requests, int32_t window, float scale,
+                         uint16_t* out, float* lse, void* workspace, size_t workspace_bytes,
+                         void* stream);
+size_t rmoe_paged_attention_workspace_bytes(const rmoe_paged_cache* cache, int32_t q_heads,
+                                            int32_t requests, int32_t table_width,
+                                            int32_t window);
+
+/* Linear attention with a decay for each head over packed sequences: rows
+ * [cu_seqlens[r], cu_seqlens[r + 1]) are sequence r's, whose state S
+ * [v heads, dk, dv] is state[i], i = state_index[r] (r itself when NULL):
+ *   S <- exp(log_decay) S + k u^T,  out = scale S^T q  (after the token)
+ *   u = v, or with beta  u = beta (v - (exp(log_decay) S)^T k)
+ * value heads [h G, (h + 1) G) use q and k head h.  The final state goes to
+ * state_out[i], which may be state.  i outside [0, slots): from zeros, and
+ * not kept.  The indices of one call differ.  log_decay, beta fp32, value
+ * (t, h) at t * row_stride + h * head_stride (0 repeats one); beta NULL: no
+ * delta rule.  out bf16 [tokens, v heads, dv]; rows of no sequence become
+ * zero with clear_uncovered and stay as they were without.  dk 64 or 128, dv
+ * a multiple of 16, v heads a multiple of k's.  States stay fp32 throughout.
+ * A NaN or infinity among a sequence's inputs may reach all of that
+ * sequence's outputs, earlier tokens' too, and no other sequence's.
+ * workspace: rmoe_linear_attention_workspace_bytes (0: the call needs none),
+ * 16-byte aligned. */
+typedef struct rmoe_gate {
+  const float* x;
+  int64_t row_stride;
+  int64_t head_stride;
+} rmoe_gate;
+int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_rows* v,
+                          const rmoe_gate* log_decay, const rmoe_gate* beta,
+                          const int32_t* cu_seqlens, int32_t tokens, int32_t requests,
+                          int32_t dk, int32_t dv, float scale, const float* state,
+                          float* state_out, const int32_t* state_index, int32_t slots,
+                          uint16_t* out, int32_t clear_uncovered, void* workspace,
+                          size_t workspace_bytes, void* stream);
+size_t rmoe_linear_attention_workspace_bytes(int32_t tokens, int32_t requests, int32_t k_heads,
+                                             int32_t v_heads, int32_t dk, int32_t delta);
 
 #ifdef __cplusplus
 }

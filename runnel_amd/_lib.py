@@ -23,7 +23,7 @@ RMOE_ENULL = -6
 RMOE_ETIMEOUT = -7
 RMOE_EPLACEMENT = -8
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 EXPORTED = (
     "rmoe_abi_version", "rmoe_last_error", "rmoe_status_string",
@@ -34,6 +34,9 @@ EXPORTED = (
     "rmoe_moe_chain", "rmoe_workspace_status_offset", "rmoe_router_q",
     "rmoe_switch_combine", "rmoe_switch_combine_workspace_bytes", "rmoe_rms_norm",
     "rmoe_set_cooperative_launch", "rmoe_moe_block_noalloc", "rmoe_combine", "rmoe_swiglu",
+    "rmoe_paged_tables", "rmoe_rotary", "rmoe_rotary_append", "rmoe_paged_attention",
+    "rmoe_paged_attention_workspace_bytes", "rmoe_linear_attention",
+    "rmoe_linear_attention_workspace_bytes",
 )
 
 # rmoe_moe_block_noalloc's static scratch per GPU (RMOE_NOALLOC_SCRATCH_BYTES)
@@ -70,6 +73,36 @@ class Layer(ctypes.Structure):
         ("router_q", QWeight), ("shared_gate_q", QWeight),
         ("post_norm_w", ctypes.c_void_p), ("norm_eps", ctypes.c_float),
     ]
+
+
+class Rows(ctypes.Structure):
+    """rmoe_rows"""
+    _fields_ = [("x", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int32)]
+
+
+class Gate(ctypes.Structure):
+    """rmoe_gate"""
+    _fields_ = [("x", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class PagedCache(ctypes.Structure):
+    """rmoe_paged_cache"""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+        ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("bits", ctypes.c_int32),
+        ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float),
+    ]
+
+
+class RotarySpec(ctypes.Structure):
+    """rmoe_rotary_spec"""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("half", ctypes.c_int32),
+                ("axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4),
+                ("woven", ctypes.c_int32), ("adjacent", ctypes.c_int32)]
 
 
 _lock = threading.Lock()
@@ -133,11 +166,29 @@ def load() -> ctypes.CDLL:
         lib.rmoe_workspace_status_offset.restype = SZ
         lib.rmoe_workspace_status_offset.argtypes = []
         lib.rmoe_set_cooperative_launch.argtypes = [I32]
+        F = ctypes.c_float
+        RP = ctypes.POINTER(Rows)
+        GP = ctypes.POINTER(Gate)
+        CP = ctypes.POINTER(PagedCache)
+        SP = ctypes.POINTER(RotarySpec)
+        lib.rmoe_paged_tables.argtypes = [P, P, I32, P, I64, I32, P, I32, I32, I32, P, P, P, P, P,
+                                          P, P]
+        lib.rmoe_rotary.argtypes = [SP, P, I64, I32, I32, RP, P, RP, P, P]
+        lib.rmoe_rotary_append.argtypes = [SP, P, I64, I32, RP, P, RP, RP, CP, P, P]
+        lib.rmoe_paged_attention.argtypes = [RP, CP, P, I64, I32, P, I32, I32, F, P, P, P, SZ, P]
+        lib.rmoe_paged_attention_workspace_bytes.restype = SZ
+        lib.rmoe_paged_attention_workspace_bytes.argtypes = [CP, I32, I32, I32, I32]
+        lib.rmoe_linear_attention.argtypes = [RP, RP, RP, GP, GP, P, I32, I32, I32, I32, F, P, P,
+                                              P, I32, P, I32, P, SZ, P]
+        lib.rmoe_linear_attention_workspace_bytes.restype = SZ
+        lib.rmoe_linear_attention_workspace_bytes.argtypes = [I32, I32, I32, I32, I32, I32]
         for name in EXPORTED:
             if name not in ("rmoe_last_error", "rmoe_status_string",
                             "rmoe_workspace_bytes", "rmoe_switch_workspace_bytes",
                             "rmoe_switch_combine_workspace_bytes",
                             "rmoe_router_workspace_bytes", "rmoe_chain_table_bytes",
+                            "rmoe_paged_attention_workspace_bytes",
+                            "rmoe_linear_attention_workspace_bytes",
                             "rmoe_workspace_status_offset"):
                 getattr(lib, name).restype = ctypes.c_int
         _lib = lib

@@ -505,6 +505,128 @@ int switch_call(const rmoe_qweight* gate_up, const rmoe_qweight* down, const uin
   return ok();
 }
 
+// ---- the token mixer
+
+int shift_of(int page_size) { return __builtin_ctz((unsigned)page_size); }
+
+// Workgroups of 256 threads that one launch may have (2^32 threads and more
+// are refused by the runtime).
+constexpr int64_t kMaxGroups = ((int64_t)1 << 24) - 1;
+
+int check_rows_of(const rmoe_rows* x, const char* name, bool used) {
+  if (!x) return fail(RMOE_ENULL, "%s: descriptor is NULL", name);
+  if (x->heads < 1 || x->heads > 65536)
+    return fail(RMOE_EINVAL, "%s: heads must be in [1, 65536] (got %d)", name, x->heads);
+  if (x->row_stride < 0 || x->head_stride < 0)
+    return fail(RMOE_EINVAL, "%s: strides must not be negative", name);
+  if (used && !x->x) return fail(RMOE_ENULL, "%s is required", name);
+  if (!aligned(x->x, 16) || x->row_stride % 8 || x->head_stride % 8)
+    return fail(RMOE_EALIGN, "%s must be 16-byte aligned, with strides of whole 16 bytes", name);
+  return RMOE_OK;
+}
+
+int check_page_size(int page_size) {
+  if (!pow2(page_size) || page_size < 8 || page_size > 1024)
+    return fail(RMOE_EINVAL, "page_size must be a power of two in [8, 1024] (got %d)", page_size);
+  return RMOE_OK;
+}
+
+int check_cache(const rmoe_paged_cache* c) {
+  if (!c) return fail(RMOE_ENULL, "cache: descriptor is NULL");
+  int rc;
+  if ((rc = check_page_size(c->page_size))) return rc;
+  if (c->dim != 64 && c->dim != 96 && c->dim != 128 && c->dim != 192 && c->dim != 256)
+    return fail(RMOE_EINVAL, "cache: dim must be 64, 96, 128, 192 or 256 (got %d)", c->dim);
+  if (c->bits != 16 && c->bits != 8)
+    return fail(RMOE_EBITS, "cache: bits must be 16 (bf16) or 8 (e4m3) (got %d)", c->bits);
+  if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 65536)
+    return fail(RMOE_EINVAL, "cache: needs a page and 1 to 65536 key heads (got %d, %d)", c->pages,
+                c->kv_heads);
+  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0)
+    return fail(RMOE_EINVAL, "cache: strides must not be negative");
+  if (!c->k || !c->v) return fail(RMOE_ENULL, "cache: k and v are required");
+  const int per16 = c->bits == 8 ? 16 : 8;
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % per16 ||
+      c->head_stride % per16 || c->row_stride % per16)
+    return fail(RMOE_EALIGN, "cache must be 16-byte aligned, with strides of whole 16 bytes");
+  if (c->bits == 8 && !(c->k_scale > 0.0f && c->v_scale > 0.0f && c->k_scale <= 3.0e38f &&
+                        c->v_scale <= 3.0e38f))
+    return fail(RMOE_EINVAL, "cache: scales must be positive and finite");
+  return RMOE_OK;
+}
+
+int check_spec(const rmoe_rotary_spec* s, int dim) {
+  if (!s) return fail(RMOE_ENULL, "rotary: descriptor is NULL");
+  if (s->half < 8 || s->half % 8 || s->half > 128 || 2 * s->half > dim)
+    return fail(RMOE_EINVAL, "half must be a multiple of 8 in [8, 128], at most dim / 2 (got %d)",
+                s->half);
+  if (s->axes < 1 || s->axes > rmoe::kMaxAxes)
+    return fail(RMOE_EINVAL, "axes must be in [1, %d] (got %d)", rmoe::kMaxAxes, s->axes);
+  int64_t sum = 0;
+  for (int x = 0; x < s->axes; ++x) {
+    if (s->sections[x] < 0) return fail(RMOE_EINVAL, "sections must not be negative");
+    if (s->woven && x > 0 && s->sections[x] > (s->half - x + s->axes - 1) / s->axes)
+      return fail(RMOE_EINVAL, "woven section %d has more pairs than its axis has turns (got %d)",
+                  x, s->sections[x]);
+    sum += s->sections[x];
+  }
+  if (sum != s->half)
+    return fail(RMOE_EINVAL, "sections must sum to half = %d (got %lld)", s->half, (long long)sum);
+  if (!s->inv_freq) return fail(RMOE_ENULL, "inv_freq is required");
+  return RMOE_OK;
+}
+
+rmoe::RotaryArgs rotary_args(const rmoe_rotary_spec* s, const int32_t* positions,
+                             int64_t axis_stride, int rows, int dim, const rmoe_rows* q,
+                             uint16_t* q_out, const rmoe_rows* k) {
+  rmoe::RotaryArgs a{};
+  a.inv_freq = s->inv_freq;
+  a.half = s->half;
+  a.axes = s->axes;
+  a.woven = s->woven != 0;
+  a.adjacent = s->adjacent != 0;
+  for (int x = 0; x < rmoe::kMaxAxes; ++x) a.sections[x] = s->sections[x];
+  a.positions = positions;
+  a.axis_stride = axis_stride;
+  a.rows = rows;
+  a.dim = dim;
+  a.q = q->x, a.q_row = q->row_stride, a.q_head = q->head_stride, a.q_heads = q->heads;
+  a.k = k->x, a.k_row = k->row_stride, a.k_head = k->head_stride, a.kv_heads = k->heads;
+  a.q_out = q_out;
+  return a;
+}
+
+int check_rotary(const rmoe_rotary_spec* s, const int32_t* positions, int64_t axis_stride, int rows,
+                 int dim, const rmoe_rows* q, const uint16_t* q_out, const rmoe_rows* k) {
+  int rc;
+  if (rows < 0 || rows > (1 << 25))
+    return fail(RMOE_EINVAL, "rows must be in [0, 2^25] (got %d)", rows);
+  if (dim < 16 || dim % 8 || dim > 1024)
+    return fail(RMOE_EINVAL, "dim must be a multiple of 8 in [16, 1024] (got %d)", dim);
+  if ((rc = check_spec(s, dim))) return rc;
+  if ((rc = check_rows_of(q, "q", rows > 0))) return rc;
+  if ((rc = check_rows_of(k, "k", rows > 0))) return rc;
+  if (rows == 0) return RMOE_OK;
+  if (!positions || !q_out) return fail(RMOE_ENULL, "positions and q_out are required");
+  if (s->axes > 1 && axis_stride < 0) return fail(RMOE_EINVAL, "axis_stride must not be negative");
+  if (!aligned(q_out, 16) || !aligned(positions, 4) || !aligned(s->inv_freq, 4))
+    return fail(RMOE_EALIGN, "q_out must be 16-byte aligned");
+  return RMOE_OK;
+}
+
+// Keys that a request of this table and window can come to, as the split
+// over workgroups goes by them.
+int64_t attention_keys(int page_size, int width, int window) {
+  const int64_t all = (int64_t)width * page_size;
+  return window > 0 && window < all ? window : all;
+}
+
+size_t attention_part_bytes(int64_t heads, int splits, int dim, size_t* ml_offset) {
+  const size_t o = (size_t)heads * splits * dim * sizeof(float);
+  if (ml_offset) *ml_offset = o;
+  return splits > 1 ? o + (size_t)heads * splits * sizeof(float2) : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -986,6 +1108,211 @@ int rmoe_set_cooperative_launch(int32_t enabled) {
   const int prev = g_cooperative.exchange(enabled ? 1 : 0);
   ok();
   return prev;
+}
+
+int rmoe_paged_tables(const int32_t* cached, const int32_t* added, int32_t requests,
+                      int32_t* block_table, int64_t table_stride, int32_t table_width,
+                      const int32_t* free_pages, int32_t free_count, int32_t page_size,
+                      int32_t rows, int64_t* slots, int32_t* positions, int32_t* request_of,
+                      int32_t* cu_seqlens, int32_t* lengths, int32_t* counts, void* stream) {
+  int rc;
+  if ((rc = check_page_size(page_size))) return rc;
+  if (requests < 1 || requests > rmoe::kMaxRequests)
+    return fail(RMOE_EINVAL, "requests must be in [1, %d] (got %d)", rmoe::kMaxRequests, requests);
+  if (table_width < 0 || table_stride < table_width || free_count < 0 || rows < 0)
+    return fail(RMOE_EINVAL, "table_width, free_count and rows must not be negative, and rows of "
+                "the table must not overlap");
+  if (!cached || !added || !cu_seqlens || !lengths || !counts)
+    return fail(RMOE_ENULL, "cached, added, cu_seqlens, lengths and counts are required");
+  if ((table_width && !block_table) || (free_count && !free_pages) ||
+      (rows && (!slots || !positions || !request_of)))
+    return fail(RMOE_ENULL, "block_table, free_pages and the rows' arrays are required");
+  if (!aligned(slots, 8)) return fail(RMOE_EALIGN, "slots must be 8-byte aligned");
+  rmoe::TableArgs a{};
+  a.cached = cached, a.added = added, a.requests = requests;
+  a.width = table_width, a.shift = shift_of(page_size);
+  a.table = block_table, a.table_stride = table_stride;
+  a.free_pages = free_pages, a.free_count = free_count;
+  a.rows = rows, a.slots = slots, a.positions = positions, a.request_of = request_of;
+  a.cu = cu_seqlens, a.lengths = lengths, a.counts = counts;
+  const hipError_t e = rmoe::launch_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "paged tables launch");
+  return ok();
+}
+
+int rmoe_rotary(const rmoe_rotary_spec* spec, const int32_t* positions, int64_t axis_stride,
+                int32_t rows, int32_t dim, const rmoe_rows* q, uint16_t* q_out,
+                const rmoe_rows* k, uint16_t* k_out, void* stream) {
+  int rc;
+  if ((rc = check_rotary(spec, positions, axis_stride, rows, dim, q, q_out, k))) return rc;
+  if (rows == 0) return ok();
+  if (!k_out) return fail(RMOE_ENULL, "k_out is required");
+  if (!aligned(k_out, 16)) return fail(RMOE_EALIGN, "k_out must be 16-byte aligned");
+  rmoe::RotaryArgs a = rotary_args(spec, positions, axis_stride, rows, dim, q, q_out, k);
+  a.k_out = k_out;
+  const hipError_t e = rmoe::launch_rotary(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "rotary launch");
+  return ok();
+}
+
+int rmoe_rotary_append(const rmoe_rotary_spec* spec, const int32_t* positions,
+                       int64_t axis_stride, int32_t rows, const rmoe_rows* q, uint16_t* q_out,
+                       const rmoe_rows* k, const rmoe_rows* v, const rmoe_paged_cache* cache,
+                       const int64_t* slots, void* stream) {
+  int rc;
+  if ((rc = check_cache(cache))) return rc;
+  if ((rc = check_rotary(spec, positions, axis_stride, rows, cache->dim, q, q_out, k))) return rc;
+  if ((rc = check_rows_of(v, "v", rows > 0))) return rc;
+  if (k->heads != cache->kv_heads || v->heads != cache->kv_heads)
+    return fail(RMOE_EINVAL, "k and v must have the cache's %d heads (got %d, %d)",
+                cache->kv_heads, k->heads, v->heads);
+  if (rows == 0) return ok();
+  if (!slots) return fail(RMOE_ENULL, "slots is required");
+  if (!aligned(slots, 8)) return fail(RMOE_EALIGN, "slots must be 8-byte aligned");
+  rmoe::RotaryArgs a = rotary_args(spec, positions, axis_stride, rows, cache->dim, q, q_out, k);
+  a.v = v->x, a.v_row = v->row_stride, a.v_head = v->head_stride;
+  a.slots = slots, a.cache_slots = (int64_t)cache->pages * cache->page_size;
+  a.k_cache = cache->k, a.v_cache = cache->v;
+  a.page_stride = cache->page_stride, a.head_stride = cache->head_stride;
+  a.row_stride = cache->row_stride;
+  a.shift = shift_of(cache->page_size), a.bits = cache->bits;
+  a.k_inv = cache->bits == 8 ? 1.0f / cache->k_scale : 1.0f;
+  a.v_inv = cache->bits == 8 ? 1.0f / cache->v_scale : 1.0f;
+  const hipError_t e = rmoe::launch_rotary(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "rotary append launch");
+  return ok();
+}
+
+size_t rmoe_paged_attention_workspace_bytes(const rmoe_paged_cache* cache, int32_t q_heads,
+                                            int32_t requests, int32_t table_width,
+                                            int32_t window) {
+  if (!cache || check_page_size(cache->page_size) || cache->kv_heads < 1 || q_heads < 1 ||
+      q_heads % cache->kv_heads || requests < 1 || table_width < 0)
+    return 0;
+  const int splits =
+      rmoe::attention_splits(requests, cache->kv_heads, q_heads / cache->kv_heads,
+                             attention_keys(cache->page_size, table_width, window));
+  return attention_part_bytes((int64_t)requests * q_heads, splits, cache->dim, nullptr);
+}
+
+int rmoe_paged_attention(const rmoe_rows* q, const rmoe_paged_cache* cache,
+                         const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                         const int32_t* lengths, int32_t requests, int32_t window, float scale,
+                         uint16_t* out, float* lse, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  int rc;
+  if ((rc = check_cache(cache))) return rc;
+  if (requests < 0 || table_width < 0 || window < 0)
+    return fail(RMOE_EINVAL, "requests, table_width and window must not be negative");
+  if ((rc = check_rows_of(q, "q", requests > 0))) return rc;
+  if (q->heads % cache->kv_heads)
+    return fail(RMOE_EINVAL, "query heads must be a multiple of the %d key heads (got %d)",
+                cache->kv_heads, q->heads);
+  if ((int64_t)table_width * cache->page_size > (1 << 30))
+    return fail(RMOE_EINVAL, "a table row may hold at most 2^30 tokens");
+  if (!(scale >= -3.0e38f && scale <= 3.0e38f))
+    return fail(RMOE_EINVAL, "scale must be finite");
+  if (requests == 0) return ok();
+  if (!lengths || !out || (table_width && !block_table))
+    return fail(RMOE_ENULL, "block_table, lengths and out are required");
+  if (!aligned(out, 16)) return fail(RMOE_EALIGN, "out must be 16-byte aligned");
+  rmoe::AttentionArgs a{};
+  a.q = q->x, a.q_row = q->row_stride, a.q_head = q->head_stride;
+  a.k_cache = cache->k, a.v_cache = cache->v;
+  a.page_stride = cache->page_stride, a.head_stride = cache->head_stride;
+  a.row_stride = cache->row_stride;
+  a.pages = cache->pages, a.shift = shift_of(cache->page_size), a.bits = cache->bits;
+  a.dim = cache->dim, a.requests = requests, a.kv_heads = cache->kv_heads;
+  a.group = q->heads / cache->kv_heads, a.head_tiles = (a.group + 15) / 16;
+  a.table = block_table, a.table_stride = table_stride, a.width = table_width;
+  a.lengths = lengths, a.window = window;
+  a.scale_log2 = scale * (a.bits == 8 ? cache->k_scale : 1.0f) * 1.44269504088896f;
+  a.v_scale = a.bits == 8 ? cache->v_scale : 1.0f;
+  a.splits = rmoe::attention_splits(requests, a.kv_heads, a.group,
+                                    attention_keys(cache->page_size, table_width, window));
+  a.out = out, a.lse = lse;
+  const int64_t heads = (int64_t)requests * q->heads;
+  if (heads > kMaxGroups ||
+      (int64_t)requests * a.kv_heads * a.head_tiles * a.splits > kMaxGroups)
+    return fail(RMOE_EINVAL, "too many requests times heads for one call");
+  size_t ml;
+  const size_t need = attention_part_bytes(heads, a.splits, a.dim, &ml);
+  if (need) {
+    if (!workspace || workspace_bytes < need)
+      return fail(RMOE_EWS, "workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
+    if (!aligned(workspace, 16)) return fail(RMOE_EALIGN, "workspace must be 16-byte aligned");
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + ml);
+  }
+  const hipError_t e = rmoe::launch_attention(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+  return ok();
+}
+
+size_t rmoe_linear_attention_workspace_bytes(int32_t tokens, int32_t requests, int32_t k_heads,
+                                             int32_t v_heads, int32_t dk, int32_t delta) {
+  if (tokens < 0 || requests < 1 || k_heads < 1 || v_heads < 1 || (dk != 64 && dk != 128)) return 0;
+  if (!rmoe::linear_in_chunks(tokens, requests)) return 0;
+  return (size_t)rmoe::linear_layout(tokens, requests, k_heads, v_heads, dk, delta != 0).total;
+}
+
+int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_rows* v,
+                          const rmoe_gate* log_decay, const rmoe_gate* beta,
+                          const int32_t* cu_seqlens, int32_t tokens, int32_t requests,
+                          int32_t dk, int32_t dv, float scale, const float* state,
+                          float* state_out, const int32_t* state_index, int32_t slots,
+                          uint16_t* out, int32_t clear_uncovered, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  int rc;
+  if (tokens < 0 || requests < 1 || slots < 0)
+    return fail(RMOE_EINVAL, "needs a sequence, and tokens and slots not negative");
+  if (dk != 64 && dk != 128) return fail(RMOE_EINVAL, "dk must be 64 or 128 (got %d)", dk);
+  if (dv < 16 || dv % 16 || dv > 1024)
+    return fail(RMOE_EINVAL, "dv must be a multiple of 16 in [16, 1024] (got %d)", dv);
+  if ((rc = check_rows_of(q, "q", tokens > 0))) return rc;
+  if ((rc = check_rows_of(k, "k", tokens > 0))) return rc;
+  if ((rc = check_rows_of(v, "v", tokens > 0))) return rc;
+  if (q->heads != k->heads || v->heads % k->heads)
+    return fail(RMOE_EINVAL, "q and k must share their heads, and v's be a multiple (got %d, %d, %d)",
+                q->heads, k->heads, v->heads);
+  if (!log_decay) return fail(RMOE_ENULL, "log_decay: descriptor is NULL");
+  if (log_decay->row_stride < 0 || log_decay->head_stride < 0 ||
+      (beta && (beta->row_stride < 0 || beta->head_stride < 0)))
+    return fail(RMOE_EINVAL, "strides must not be negative");
+  if (!(scale >= -3.0e38f && scale <= 3.0e38f)) return fail(RMOE_EINVAL, "scale must be finite");
+  if (!cu_seqlens || (slots && (!state || !state_out)))
+    return fail(RMOE_ENULL, "cu_seqlens, state and state_out are required");
+  if (tokens && (!log_decay->x || (beta && !beta->x) || !out))
+    return fail(RMOE_ENULL, "log_decay, beta's values and out are required");
+  if (!aligned(state, 16) || !aligned(state_out, 16) || !aligned(out, 16))
+    return fail(RMOE_EALIGN, "state, state_out and out must be 16-byte aligned");
+  rmoe::LinearArgs a{};
+  a.q = q->x, a.q_row = q->row_stride, a.q_head = q->head_stride;
+  a.k = k->x, a.k_row = k->row_stride, a.k_head = k->head_stride;
+  a.v = v->x, a.v_row = v->row_stride, a.v_head = v->head_stride;
+  a.decay = log_decay->x, a.decay_row = log_decay->row_stride;
+  a.decay_head = log_decay->head_stride;
+  if (beta) a.beta = beta->x, a.beta_row = beta->row_stride, a.beta_head = beta->head_stride;
+  a.delta = beta != nullptr;
+  a.cu = cu_seqlens, a.tokens = tokens, a.requests = requests;
+  a.k_heads = k->heads, a.v_heads = v->heads, a.dk = dk, a.dv = dv, a.scale = scale;
+  a.state = state, a.state_out = state_out, a.index = state_index, a.slots = slots;
+  a.out = out, a.clear = clear_uncovered != 0 && tokens > 0;
+  const rmoe::LinearLayout l =
+      rmoe::linear_layout(tokens, requests, a.k_heads, a.v_heads, dk, a.delta);
+  const int64_t tiles = (int64_t)requests * a.v_heads * (dv / 16);
+  if (tiles + 8 * 64 > kMaxGroups || l.chunks * a.v_heads + 64 > kMaxGroups)
+    return fail(RMOE_EINVAL, "too many sequences, tokens or heads for one call");
+  if (rmoe::linear_in_chunks(tokens, requests)) {
+    if (!workspace || workspace_bytes < (size_t)l.total)
+      return fail(RMOE_EWS, "workspace of %zu bytes needed (got %zu)", (size_t)l.total,
+                  workspace_bytes);
+    if (!aligned(workspace, 16)) return fail(RMOE_EALIGN, "workspace must be 16-byte aligned");
+    a.workspace = workspace, a.chunks = l.chunks, a.kt_offset = l.kt_offset;
+  }
+  const hipError_t e = rmoe::launch_linear(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "linear attention launch");
+  return ok();
 }
 
 int rmoe_stream_read(const void* buffer, size_t bytes, uint32_t* partials,

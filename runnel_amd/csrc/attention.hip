@@ -1,0 +1,510 @@
+// Attention of one new token of each request over its paged cache.
+//
+//   o_h = sum_j p_hj v_j / sum_j p_hj,  p_hj = exp(scale q_h . k_j - m_h)
+//
+// over the keys j of [length - window, length).  Bound by the read of K and
+// V (2 bytes, or one, of each are used in at most `group` products), so the
+// kernel is built around keeping loads in flight: K and V go from memory
+// straight into the registers that feed the matrix instructions, with no
+// LDS pass and no barrier before the end.
+//
+//   - 16 query heads of one key head (the group, padded) times 32 keys a
+//     step: scores^T = K Q^T as 16x16x32 products, key rows as operand A.
+//   - scores^T leaves lane (g, n) with keys 4 g + i of head n in each 16-key
+//     half, which is just the operand layout of the second product with its
+//     contraction index permuted (index 8 g + 4 half + i is key 16 half +
+//     4 g + i), so the probabilities never move between lanes.
+//   - out^T = V^T P^T: lane (g, n) loads for its 8 keys the dims n E ..
+//     n E + E - 1 (E = 8 of 128: whole lines of V) and transposes them among
+//     its own registers with byte permutes; tile e's row m is dim m E + e.
+//   - running maximum and sum per head, in base 2 with the scale folded in.
+//     The probabilities are rounded to bf16 for the second product (half a
+//     step, 2^-9, of numbers that are averaged; the sum is of the unrounded
+//     ones); everything else is fp32.
+//
+// A request's keys are split over several workgroups and, in each, over its
+// four waves; a second launch joins the workgroups' parts in their order.
+#include <type_traits>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace rmoe {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kAttThreads = 256;
+constexpr int kAttWaves = kAttThreads / kWave;
+constexpr int kAttTile = 32;  // keys of a step
+constexpr float kLn2 = 0.69314718056f;
+
+__device__ __forceinline__ bf16x8 frag(const uint32_t (&w)[4]) {
+  union {
+    uint32_t w[4];
+    bf16x8 v;
+  } u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u.w[i] = w[i];
+  return u.v;
+}
+
+__device__ __forceinline__ f32x4 mfma(const bf16x8 a, const bf16x8 b, const f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Maximum / sum over the four lanes that hold one head (l ^ 16, l ^ 32).
+__device__ __forceinline__ float head_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float head_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  union {
+    bf16x2 v;
+    uint32_t u;
+  } r;
+  r.v = __builtin_convertvector((f32x2){lo, hi}, bf16x2);
+  return r.u;
+}
+
+// Two e4m3 values (the low or high half of w) as packed bf16: exact.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t w) {
+  union {
+    bf16x2 v;
+    uint32_t u;
+  } r;
+  r.v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH);
+  return r.u;
+}
+
+// BYTES consecutive bytes (2, 4, 8, 16) as dwords.
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+  if constexpr (BYTES == 16) {
+    const uint4 u = load16(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    static_assert(BYTES == 2, "2, 4, 8 or 16 bytes");
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  }
+}
+
+// A head's dims as runs of 128, 64 or 32: lane n of 16 holds P / 16
+// consecutive ones of each run.
+template <int D>
+struct Runs {
+  static constexpr int first = D >= 128 ? 128 : 64;
+  static constexpr int second = D - first;
+};
+
+// What the split of a request comes to: its keys [start, end), the tiles of
+// 32 they touch, and how many of them each workgroup takes.
+struct Share {
+  int start, end;   // keys
+  int tile0;        // first tile
+  int tiles;        // of the request
+  int per;          // of a workgroup
+  int parts;        // workgroups with work
+};
+
+__device__ __forceinline__ Share share_of(const AttentionArgs& a, int r) {
+  Share s;
+  const int64_t most = (int64_t)a.width << a.shift;
+  const int len = (int)(a.lengths[r] < most ? a.lengths[r] : most);
+  s.end = len > 0 ? len : 0;
+  s.start = a.window > 0 && s.end > a.window ? s.end - a.window : 0;
+  s.tile0 = s.start / kAttTile;
+  s.tiles = s.end > s.start ? (s.end - 1) / kAttTile + 1 - s.tile0 : 0;
+  // no workgroup under a.least tiles while there is another
+  int want = (s.tiles + a.least - 1) / a.least;
+  want = want < a.splits ? want : a.splits;
+  want = want > 0 ? want : 1;
+  s.per = (s.tiles + want - 1) / want;
+  s.parts = s.per ? (s.tiles + s.per - 1) / s.per : 0;
+  return s;
+}
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kAttThreads, D > 128 && !E4M3 ? 1 : 2) void attention_kernel(
+    const AttentionArgs a) {
+  constexpr int EB = E4M3 ? 1 : 2;    // bytes of a cached value
+  constexpr int KS = D / 32;          // steps of the first product
+  constexpr int NT = D / 16;          // tiles of the second
+  constexpr int P0 = Runs<D>::first, P1 = Runs<D>::second;
+  constexpr int E0 = P0 / 16, E1 = P1 / 16;
+  constexpr int V0 = (E0 * EB + 3) / 4, V1 = (E1 * EB + 3) / 4;  // dwords of a key's runs
+  constexpr int KW = KS * 8 * EB / 4;                            // dwords of a key's share
+  extern __shared__ float lds[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  // (split, head tile, key head, request), the request slowest
+  int b = blockIdx.x;
+  const int split = b % a.splits;
+  b /= a.splits;
+  const int ht = b % a.head_tiles;
+  b /= a.head_tiles;
+  const int hk = b % a.kv_heads;
+  const int r = b / a.kv_heads;
+  const Share sh = share_of(a, r);
+  const int t_begin = split * sh.per;
+  const int t_end = t_begin + sh.per < sh.tiles ? t_begin + sh.per : sh.tiles;
+  if (split > 0 && t_begin >= sh.tiles) return;
+
+  const int left = a.group - ht * 16;
+  const int heads = left < 16 ? left : 16;  // of this workgroup
+  const int head0 = hk * a.group + ht * 16;
+
+  // queries, operand B: head n, the dims of each step as the keys have them
+  bf16x8 qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    int d = 32 * s + 8 * g;
+    if (E4M3 && (s | 1) < KS) d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+    if (n < heads) {
+      const uint16_t* p = a.q + (int64_t)r * a.q_row + (int64_t)(head0 + n) * a.q_head + d;
+      const uint4 u = load16(p);
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    }
+    qf[s] = frag(w);
+  }
+
+  const uint8_t* kc = static_cast<const uint8_t*>(a.k_cache) + (int64_t)hk * a.head_stride * EB;
+  const uint8_t* vc = static_cast<const uint8_t*>(a.v_cache) + (int64_t)hk * a.head_stride * EB;
+  const int32_t* table = a.table + r * a.table_stride;
+  const int in_page = (1 << a.shift) - 1;
+  const int last = sh.end - 1;
+
+  // page numbers of tile t: of key 16 half + n for K, of the four keys
+  // 16 half + 4 g .. for V.  Keys past the end look the last key's page up.
+  auto pages = [&](int t, int (&pk)[2], int (&pv)[2]) {
+    const int key0 = (sh.tile0 + t) * kAttTile;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int jk = key0 + 16 * h + n, jv = key0 + 16 * h + 4 * g;
+      pk[h] = table[(jk < last ? jk : last) >> a.shift];
+      pv[h] = table[(jv < last ? jv : last) >> a.shift];
+    }
+  };
+  // a page that is none of the cache's is read as page 0 and masked
+  auto row_of = [&](int page, int key) {
+    const int64_t p = (uint32_t)page < (uint32_t)a.pages ? page : 0;
+    return (p * a.page_stride + (int64_t)(key & in_page) * a.row_stride) * EB;
+  };
+  uint32_t kw[2][KW];
+  uint32_t v0[8][V0], v1[8][V1 ? V1 : 1];
+  auto load_k = [&](int t, const int (&pk)[2]) {
+    const int key0 = (sh.tile0 + t) * kAttTile;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* p = kc + row_of(pk[h], key0 + 16 * h + n);
+      if constexpr (!E4M3) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) load_bytes<16>(p + (32 * s + 8 * g) * 2, &kw[h][4 * s]);
+      } else {
+#pragma unroll
+        for (int s = 0; s + 1 < KS; s += 2) load_bytes<16>(p + 32 * s + 16 * g, &kw[h][2 * s]);
+        if constexpr (KS & 1) load_bytes<8>(p + 32 * (KS - 1) + 8 * g, &kw[h][2 * (KS - 1)]);
+      }
+    }
+  };
+  auto load_v = [&](int t, const int (&pv)[2]) {
+    const int key0 = (sh.tile0 + t) * kAttTile;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* p = vc + row_of(pv[j >> 2], key0 + 16 * (j >> 2) + 4 * g + (j & 3));
+      load_bytes<E0 * EB>(p + n * E0 * EB, v0[j]);
+      if constexpr (P1 > 0) load_bytes<E1 * EB>(p + (P0 + n * E1) * EB, v1[j]);
+    }
+  };
+
+  f32x4 o[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+
+  int t = t_begin + wave;
+  int pk[2], pv[2];
+  if (t < t_end) {
+    pages(t, pk, pv);
+    load_k(t, pk);
+    load_v(t, pv);
+  }
+  for (; t < t_end; t += kAttWaves) {
+    const int next = t + kAttWaves;
+    const int now_v[2] = {pv[0], pv[1]};
+    if (next < t_end) pages(next, pk, pv);
+
+    f32x4 sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        uint32_t w[4];
+        if constexpr (!E4M3) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = kw[h][4 * s + i];
+        } else {
+          w[0] = e4m3_to_bf16<false>(kw[h][2 * s]);
+          w[1] = e4m3_to_bf16<true>(kw[h][2 * s]);
+          w[2] = e4m3_to_bf16<false>(kw[h][2 * s + 1]);
+          w[3] = e4m3_to_bf16<true>(kw[h][2 * s + 1]);
+        }
+        sc[h] = mfma(frag(w), qf[s], sc[h]);
+      }
+    }
+    if (next < t_end) load_k(next, pk);
+
+    // keys outside the request's or without a page: no weight, and their
+    // values cleared, since 0 times a leftover infinity or NaN is NaN
+    const int key0 = (sh.tile0 + t) * kAttTile;
+    const bool bad_page = (uint32_t)now_v[0] >= (uint32_t)a.pages ||
+                          (uint32_t)now_v[1] >= (uint32_t)a.pages;
+    const bool edge = key0 < sh.start || key0 + kAttTile > sh.end || __any(bad_page);
+    uint32_t dead = 0;
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+        if (key < sh.start || key >= sh.end || (uint32_t)now_v[j >> 2] >= (uint32_t)a.pages)
+          dead |= 1u << j;
+      }
+    }
+    float x[8];
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = sc[j >> 2][j & 3] * a.scale_log2;
+      if (edge && (dead >> j & 1)) x[j] = -INFINITY;
+      top = fmaxf(top, x[j]);
+    }
+    top = fmaxf(m, head_max(top));
+    if (__any(top > m)) {
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float shrink = __builtin_amdgcn_exp2f(m - base);
+      l *= shrink;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[i] *= shrink;
+      m = top;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    uint32_t pw[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+      l += x[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pw[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+    const bf16x8 pf = frag(pw);
+
+    // bf16 values of a run of key j, then the transposed fragments
+    auto second = [&](const uint32_t* raw, int j, int dw) -> uint32_t {
+      // dword dw (dims 2 dw, 2 dw + 1 of the lane's run) of key j as bf16
+      uint32_t w;
+      if constexpr (E4M3) {
+        w = dw & 1 ? e4m3_to_bf16<true>(raw[dw >> 1]) : e4m3_to_bf16<false>(raw[dw >> 1]);
+      } else {
+        w = raw[dw];
+      }
+      return edge && (dead >> j & 1) ? 0u : w;
+    };
+#pragma unroll
+    for (int dw = 0; dw < E0 / 2; ++dw) {
+      uint32_t w[8], lo[4], hi[4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = second(v0[j], j, dw);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100);
+        hi[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302);
+      }
+      o[2 * dw] = mfma(frag(lo), pf, o[2 * dw]);
+      o[2 * dw + 1] = mfma(frag(hi), pf, o[2 * dw + 1]);
+    }
+    if constexpr (P1 > 0) {
+#pragma unroll
+      for (int dw = 0; dw < E1 / 2; ++dw) {
+        uint32_t w[8], lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = second(v1[j], j, dw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100);
+          hi[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302);
+        }
+        o[E0 + 2 * dw] = mfma(frag(lo), pf, o[E0 + 2 * dw]);
+        o[E0 + 2 * dw + 1] = mfma(frag(hi), pf, o[E0 + 2 * dw + 1]);
+      }
+    }
+    if (next < t_end) load_v(next, pv);
+  }
+
+  // the four waves' parts together, a run of dims at a time
+  l = head_sum(l);
+  float* ml = lds + kAttWaves * heads * P0;  // [wave][head] maximum, then sum
+  if (n < heads && g == 0) {
+    ml[wave * 16 + n] = m;
+    ml[(kAttWaves + wave) * 16 + n] = l;
+  }
+  const int64_t row = (int64_t)r * a.kv_heads * a.group + head0;
+  auto join = [&](auto run) {
+    constexpr int P = decltype(run)::value ? P1 : P0, E = P / 16;
+    constexpr int I0 = decltype(run)::value ? E0 : 0, D0 = decltype(run)::value ? P0 : 0;
+    if (n < heads) {
+      float* mine = lds + (wave * heads + n) * P + 4 * g * E;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mine[k * E + i] = o[I0 + i][k];
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * P; i += kAttThreads) {
+      const int h = i / P, d = i - h * P;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kAttWaves; ++w) top = fmaxf(top, ml[w * 16 + h]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kAttWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ml[w * 16 + h] - base);
+        sum += f * ml[(kAttWaves + w) * 16 + h];
+        acc += f * lds[(w * heads + h) * P + d];
+      }
+      if (a.splits == 1) {
+        const bool some = sum > 0.0f || sum != sum;
+        a.out[(row + h) * D + D0 + d] =
+            (uint16_t)f32_to_bf16(some ? acc / sum * a.v_scale : 0.0f);
+        if (a.lse && D0 + d == 0)
+          a.lse[row + h] = top == -INFINITY ? top : (top + log2f(sum)) * kLn2;
+      } else {
+        const int64_t part = (row + h) * a.splits + split;
+        a.part_o[part * D + D0 + d] = acc;
+        if (D0 + d == 0) a.part_ml[part] = make_float2(top, sum);
+      }
+    }
+  };
+  join(std::integral_constant<int, 0>());
+  if constexpr (P1 > 0) {
+    __syncthreads();
+    join(std::integral_constant<int, 1>());
+  }
+}
+
+// Joins the parts of one head: 256 threads, D / 4 of them across the dims
+// and the rest across the parts.
+template <int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs a) {
+  constexpr int C = D / 4;          // threads across the dims
+  constexpr int Q = 256 / C;        // parts at a time
+  __shared__ float4 acc_s[Q][C];
+  __shared__ float sum_s[Q];
+  const int64_t row = blockIdx.x;  // request and head
+  const int heads = a.kv_heads * a.group;
+  const Share sh = share_of(a, (int)(row / heads));
+  const int tid = threadIdx.x, c = tid % C, q = tid / C;
+  float top = -INFINITY;
+  const float2* ml = a.part_ml + row * a.splits;
+  for (int i = tid & 63; i < sh.parts; i += 64) top = fmaxf(top, ml[i].x);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float sum = 0.0f;
+  if (q < Q) {
+#pragma unroll 4
+    for (int i = q; i < sh.parts; i += Q) {
+      const float2 e = ml[i];
+      const float f = __builtin_amdgcn_exp2f(e.x - base);
+      const float4 v = reinterpret_cast<const float4*>(a.part_o + (row * a.splits + i) * D)[c];
+      sum += f * e.y;
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    }
+    acc_s[q][c] = acc;
+    if (c == 0) sum_s[q] = sum;
+  }
+  __syncthreads();
+  if (tid >= C) return;
+  acc = acc_s[0][c];
+  sum = sum_s[0];
+#pragma unroll
+  for (int i = 1; i < Q; ++i) {
+    const float4 v = acc_s[i][c];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    sum += sum_s[i];
+  }
+  const bool some = sum > 0.0f || sum != sum;
+  const float f = some ? a.v_scale / sum : 0.0f;
+  uint2 w;
+  w.x = f32_to_bf16(some ? acc.x * f : 0.0f) | f32_to_bf16(some ? acc.y * f : 0.0f) << 16;
+  w.y = f32_to_bf16(some ? acc.z * f : 0.0f) | f32_to_bf16(some ? acc.w * f : 0.0f) << 16;
+  reinterpret_cast<uint2*>(a.out + row * D)[c] = w;
+  if (a.lse && tid == 0) a.lse[row] = top == -INFINITY ? top : (top + log2f(sum)) * kLn2;
+}
+
+template <int D, bool E4M3>
+hipError_t launch_attention_of(const AttentionArgs& a, hipStream_t s) {
+  const int heads = a.group < 16 ? a.group : 16;
+  const size_t lds = (size_t)(kAttWaves * heads * Runs<D>::first + 2 * kAttWaves * 16) * sizeof(float);
+  const int64_t grid = (int64_t)a.requests * a.kv_heads * a.head_tiles * a.splits;
+  attention_kernel<D, E4M3><<<(unsigned)grid, kAttThreads, lds, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  attention_join_kernel<D><<<(unsigned)(a.requests * a.kv_heads * a.group), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_attention_dim(const AttentionArgs& a, hipStream_t s) {
+  return a.bits == 8 ? launch_attention_of<D, true>(a, s) : launch_attention_of<D, false>(a, s);
+}
+
+}  // namespace
+
+int attention_splits(int requests, int kv_heads, int group, int64_t keys) {
+  // two workgroups a compute unit where there are keys for them (a
+  // workgroup's four waves take a tile each at least)
+  const int64_t base = (int64_t)requests * kv_heads * ((group + 15) / 16);
+  const int64_t tiles = (keys + kAttTile - 1) / kAttTile;
+  int64_t want = (512 + base - 1) / base;
+  const int64_t most = (tiles + kAttWaves - 1) / kAttWaves;
+  want = want < most ? want : most;
+  return (int)(want < 1 ? 1 : want);
+}
+
+hipError_t launch_attention(const AttentionArgs& in, hipStream_t s) {
+  AttentionArgs a = in;
+  a.least = kAttWaves;  // a tile for each wave
+  switch (a.dim) {
+    case 64: return launch_attention_dim<64>(a, s);
+    case 96: return launch_attention_dim<96>(a, s);
+    case 128: return launch_attention_dim<128>(a, s);
+    case 192: return launch_attention_dim<192>(a, s);
+    default: return launch_attention_dim<256>(a, s);
+  }
+}
+
+}  // namespace rmoe

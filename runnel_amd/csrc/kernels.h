@@ -211,4 +211,93 @@ bool dense_qmm_eligible(int M, int N, int K);
 hipError_t launch_dense_qmm(const uint16_t* x, int M, const QW& w, int N, int K, int bits,
                             uint16_t* y, hipStream_t s);
 
+// ---- the token mixer's operators (paged.hip, attention.hip, linear.hip).
+constexpr int kMaxRequests = 4096;  // of one rmoe_paged_tables call
+constexpr int kMaxAxes = 4;
+
+struct TableArgs {
+  const int32_t* cached;      // [requests]
+  const int32_t* added;       // [requests]
+  int requests, width, shift;  // width: pages of a row; a page holds 1 << shift tokens
+  int32_t* table;             // [requests, width]
+  int64_t table_stride;
+  const int32_t* free_pages;  // [free_count]
+  int free_count, rows;
+  int64_t* slots;             // [rows]
+  int32_t* positions;         // [rows]
+  int32_t* request_of;        // [rows]
+  int32_t* cu;                // [requests + 1]
+  int32_t* lengths;           // [requests]
+  int32_t* counts;            // [3]
+};
+hipError_t launch_tables(const TableArgs& a, hipStream_t s);
+
+// Strides in values.  slots NULL: the rotated keys go to k_out.
+struct RotaryArgs {
+  const float* inv_freq;      // [half]
+  int half, axes, woven, adjacent;
+  int sections[kMaxAxes];
+  const int32_t* positions;   // [axes, rows]
+  int64_t axis_stride, rows;
+  int dim, q_heads, kv_heads;
+  const uint16_t *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  uint16_t *q_out, *k_out;    // [rows, heads, dim]
+  const int64_t* slots;       // [rows]
+  int64_t cache_slots;
+  void *k_cache, *v_cache;
+  int64_t page_stride, head_stride, row_stride;
+  int shift, bits;
+  float k_inv, v_inv;
+};
+hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
+
+struct AttentionArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  const void *k_cache, *v_cache;
+  int64_t page_stride, head_stride, row_stride;
+  int pages, shift, bits, dim;
+  int requests, kv_heads, group, head_tiles;  // group: query heads of a key head
+  const int32_t* table;
+  int64_t table_stride;
+  int width;
+  const int32_t* lengths;
+  int window;                 // 0: all keys
+  float scale_log2, v_scale;  // k's scale and log2(e) are in the first
+  int splits, least;          // workgroups of a request, tiles of each at least
+  uint16_t* out;              // [requests, kv_heads * group, dim]
+  float* lse;                 // [requests, heads] or NULL
+  float* part_o;              // [requests, heads, splits, dim] (splits > 1)
+  float2* part_ml;            // [requests, heads, splits]
+};
+int attention_splits(int requests, int kv_heads, int group, int64_t keys);
+hipError_t launch_attention(const AttentionArgs& a, hipStream_t s);
+
+struct LinearArgs {
+  const uint16_t *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const float *decay, *beta;
+  int delta;                  // the delta rule, with beta
+  int64_t decay_row, decay_head, beta_row, beta_head;
+  const int32_t* cu;          // [requests + 1]
+  int tokens, requests, k_heads, v_heads, dk, dv;
+  float scale;
+  const float* state;
+  float* state_out;           // [slots, v_heads, dk, dv]
+  const int32_t* index;       // [requests] or NULL
+  int64_t slots;
+  uint16_t* out;              // [tokens, v_heads, dv]
+  int clear;                  // rows of no sequence are set to zero
+  void* workspace;            // NULL: token by token
+  int64_t chunks, kt_offset;
+};
+struct LinearLayout {
+  int64_t chunks, kt_offset, total;
+};
+bool linear_in_chunks(int64_t tokens, int requests);
+LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_heads, int dk,
+                           bool delta);
+hipError_t launch_linear(const LinearArgs& a, hipStream_t s);
+
 }  // namespace rmoe

@@ -690,6 +690,321 @@ def dequantize(weight, scales, biases, bits: int, group_size: int = 64,
     return out
 
 
+# ------------------------------------------------------- the token mixer
+# The decoder layer's other half: the paged key-value cache's bookkeeping,
+# rotary positions written through to it, attention of one new token over
+# it, and linear attention over a recurrent state.  None of these keeps
+# anything between calls: their scratch comes from torch's allocator for each
+# call, so calls on several streams and captured graphs share nothing.
+
+E4M3 = torch.float8_e4m3fn
+
+
+def _one_device(*tensors) -> torch.device:
+    """The GPU all of the tensors are on; refuses tensors that want a gradient
+    (the operators below have no backward pass)."""
+    device = None
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("runnel_amd kernels take GPU tensors")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"tensors are on {device} and {t.device}")
+        if grad and t.requires_grad:
+            raise ValueError("this operator has no backward pass: call it under torch.no_grad() "
+                             "or on detached tensors")
+    return device
+
+
+def _there(device: torch.device):
+    """Makes `device` the current one for a launch."""
+    return torch.cuda.device(device.index)
+
+
+def _int32(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise ValueError(f"{name} must be int32 (got {t.dtype})")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+    return t.to(torch.int32).contiguous()
+
+
+def _heads(t: torch.Tensor, name: str, rows: int | None = None, heads: int | None = None,
+           dim: int | None = None):
+    """A bf16 [rows, heads, dim] tensor and its rmoe_rows: as it lies where the
+    kernels can read it so (a slice of a packed projection), else copied."""
+    if t.dtype != BF16 or t.dim() != 3:
+        raise ValueError(f"{name} must be a bfloat16 [rows, heads, dim] tensor "
+                         f"(got {t.dtype} {list(t.shape)})")
+    want = (t.shape[0] if rows is None else rows, t.shape[1] if heads is None else heads,
+            t.shape[2] if dim is None else dim)
+    if tuple(t.shape) != want:
+        raise ValueError(f"{name} must be {list(want)} (got {list(t.shape)})")
+    if (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+        t = t.clone(memory_format=torch.contiguous_format)
+        if t.stride(0) % 8 or t.stride(1) % 8:
+            raise ValueError(f"{name}'s dim must be a multiple of 8 (got {t.shape[2]})")
+    return t, _lib.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1])
+
+
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: float,
+           v_scale: float) -> _lib.PagedCache:
+    if k_cache.dtype not in (BF16, E4M3):
+        raise ValueError(f"the cache must be bfloat16 or float8_e4m3fn (got {k_cache.dtype})")
+    if k_cache.dim() != 4:
+        raise ValueError("the cache must be [pages, kv heads, page size, dim] "
+                         f"(got {list(k_cache.shape)})")
+    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache and v_cache must have one type and shape")
+    pages, heads, size, dim = k_cache.shape
+    # (a dimension of one has no stride)
+    ks, vs = ([0 if n == 1 else st for n, st in zip(c.shape, c.stride())]
+              for c in (k_cache, v_cache))
+    if ks != vs:
+        raise ValueError("k_cache and v_cache must lie in memory alike")
+    if ks[3] != 1:
+        raise ValueError("the cache's last dimension must be contiguous")
+    eight = k_cache.dtype == E4M3
+    if not eight and (k_scale != 1.0 or v_scale != 1.0):
+        raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages,
+                           size, heads, dim, 8 if eight else 16, k_scale, v_scale)
+
+
+@dataclass
+class PagedTables:
+    """What ``paged_tables`` makes of a step: per row (token) its ``slots``
+    (int64, -1: none), ``positions`` and ``requests`` (int32), per request
+    ``cu_seqlens`` (int32 [R + 1]) and ``lengths`` (int32), and ``counts``
+    (int32: tokens, pages taken, pages missing)."""
+    slots: torch.Tensor
+    positions: torch.Tensor
+    requests: torch.Tensor
+    cu_seqlens: torch.Tensor
+    lengths: torch.Tensor
+    counts: torch.Tensor
+
+
+def paged_tables(cached: torch.Tensor, added: torch.Tensor, block_table: torch.Tensor,
+                 free_pages: torch.Tensor, page_size: int, rows: int) -> PagedTables:
+    """One serving step's bookkeeping from lengths on the GPU, without a copy
+    to the host.  cached / added int [R] (R <= 4096): tokens each request holds
+    and takes in this step; block_table int32 [R, P], updated in place: the
+    pages that requests grow into come from free_pages (int32 [F]) in order,
+    -1 once these are used up (``counts[2]`` then says how many were missing;
+    the caller takes ``counts[1]`` pages off the list's front).  `rows` is the
+    row count of the step's batch: tokens of all requests one after the
+    other, rows behind the last one marked -1."""
+    lib = _lib.load()
+    device = _one_device(cached, added, block_table, free_pages)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise ValueError("block_table must be int32 [requests, pages]")
+    R, P = block_table.shape
+    if P > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table's rows must be contiguous (it is updated in place)")
+    cached, added = _int32(cached, "cached", (R,)), _int32(added, "added", (R,))
+    free_pages = _int32(free_pages, "free_pages", (free_pages.numel(),))
+    if rows < 0:
+        raise ValueError(f"rows must not be negative (got {rows})")
+    ints = torch.empty(2 * rows + 2 * R + 4, dtype=torch.int32, device=device)
+    positions, requests, cu, lengths, counts = ints.split([rows, rows, R + 1, R, 3])
+    slots = torch.empty(rows, dtype=torch.int64, device=device)
+    with _there(device):
+        _lib.check(lib.rmoe_paged_tables(
+            cached.data_ptr(), added.data_ptr(), R, block_table.data_ptr(),
+            max(block_table.stride(0), P) if R == 1 else block_table.stride(0), P,
+            free_pages.data_ptr(), free_pages.numel(), page_size, rows, slots.data_ptr(),
+            positions.data_ptr(), requests.data_ptr(), cu.data_ptr(), lengths.data_ptr(),
+            counts.data_ptr(), _lib.stream_handle(device)))
+    return PagedTables(slots, positions, requests, cu, lengths, counts)
+
+
+def _rotary_spec(inv_freq, positions, rows: int, sections, woven: bool, adjacent: bool):
+    """(rmoe_rotary_spec, positions int32 [axes, rows], its axis stride)."""
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float32 vector")
+    half = inv_freq.numel()
+    sections = (half,) if sections is None else tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 4:
+        raise ValueError(f"sections must name 1 to 4 axes (got {len(sections)})")
+    if positions.dim() == 1:
+        positions = positions[None]
+    positions = _int32(positions, "positions", (len(sections), rows))
+    spec = _lib.RotarySpec(inv_freq.data_ptr(), half, len(sections),
+                           (ctypes.c_int32 * 4)(*sections), int(bool(woven)),
+                           int(bool(adjacent)))
+    return spec, positions
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+           sections=None, woven: bool = False, adjacent: bool = False):
+    """Rotary positions of one to four axes: q bf16 [N, Hq, D], k bf16 [N, Hk,
+    D] -> the turned (q, k).  The first 2 * len(inv_freq) values of a head
+    turn, pair i by positions[axis(i)] * inv_freq[i] (float32; the angle is
+    made in 64 bits); pairs are (i, i + len(inv_freq)), or neighbours when
+    `adjacent`.  positions int [N], or [A, N] with `sections`, A counts of
+    pairs that sum to len(inv_freq): the axes one section after the other, or
+    in turn when `woven` (axis i mod A until its section is used up, axis 0
+    beyond)."""
+    lib = _lib.load()
+    device = _one_device(q, k, positions, inv_freq)
+    q, qr = _heads(q, "q")
+    k, kr = _heads(k, "k", q.shape[0], None, q.shape[2])
+    spec, positions = _rotary_spec(inv_freq, positions, q.shape[0], sections, woven, adjacent)
+    q_out = torch.empty(q.shape, dtype=BF16, device=device)
+    k_out = torch.empty(k.shape, dtype=BF16, device=device)
+    with _there(device):
+        _lib.check(lib.rmoe_rotary(
+            ctypes.byref(spec), positions.data_ptr(), positions.stride(0), q.shape[0], q.shape[2],
+            ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), k_out.data_ptr(),
+            _lib.stream_handle(device)))
+    return q_out, k_out
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                  inv_freq: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slots: torch.Tensor, sections=None, woven: bool = False,
+                  adjacent: bool = False, k_scale: float = 1.0,
+                  v_scale: float = 1.0) -> torch.Tensor:
+    """``rotary`` with the turned keys and the values v bf16 [N, Hk, D] written
+    into the paged cache (bf16 or float8_e4m3fn [pages, Hk, page size, D], any
+    strides with contiguous last dimension) at slots int64 [N] (page * page
+    size + place, as ``paged_tables`` gives them; -1: nowhere) -> the turned q.
+    8-bit caches hold e4m3(x / scale), saturating.  Slots of one call differ."""
+    lib = _lib.load()
+    device = _one_device(q, k, v, positions, inv_freq, k_cache, v_cache, slots)
+    cache = _cache(k_cache, v_cache, k_scale, v_scale)
+    for n, st in zip(k_cache.shape, k_cache.stride()):
+        if n > 1 and st == 0:
+            raise ValueError("an expanded cache cannot be written")
+    q, qr = _heads(q, "q", None, None, cache.dim)
+    N = q.shape[0]
+    k, kr = _heads(k, "k", N, cache.kv_heads, cache.dim)
+    v, vr = _heads(v, "v", N, cache.kv_heads, cache.dim)
+    spec, positions = _rotary_spec(inv_freq, positions, N, sections, woven, adjacent)
+    if slots.dtype != torch.int64 or tuple(slots.shape) != (N,):
+        raise ValueError(f"slots must be int64 [{N}] (got {slots.dtype} {list(slots.shape)})")
+    slots = slots.contiguous()
+    q_out = torch.empty(q.shape, dtype=BF16, device=device)
+    with _there(device):
+        _lib.check(lib.rmoe_rotary_append(
+            ctypes.byref(spec), positions.data_ptr(), positions.stride(0), N, ctypes.byref(qr),
+            q_out.data_ptr(), ctypes.byref(kr), ctypes.byref(vr), ctypes.byref(cache),
+            slots.data_ptr(), _lib.stream_handle(device)))
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: float | None = None, window: int = 0, k_scale: float = 1.0,
+                    v_scale: float = 1.0, return_lse: bool = False):
+    """Attention of one new token of each request over its paged cache:
+    q bf16 [R, Hq, D], caches as for ``rotary_append``, block_table int32
+    [R, P] of page numbers, lengths int [R] (keys, the new token's own among
+    them) -> bf16 [R, Hq, D].  scale defaults to D ** -0.5; window > 0 leaves
+    the last `window` keys of each request; query heads share key heads in
+    order (Hq a multiple of Hk).  Keys of a page outside the cache (-1) do not
+    count.  A request without keys gets zeros.  With return_lse also float32
+    [R, Hq], the logarithm of the sum of the exponentials (-inf: no keys)."""
+    lib = _lib.load()
+    device = _one_device(q, k_cache, v_cache, block_table, lengths)
+    cache = _cache(k_cache, v_cache, k_scale, v_scale)
+    q, qr = _heads(q, "q", None, None, cache.dim)
+    R, heads, D = q.shape
+    if block_table.dim() != 2 or block_table.shape[0] != R:
+        raise ValueError(f"block_table must be [{R}, pages] (got {list(block_table.shape)})")
+    if block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        block_table = _int32(block_table, "block_table", block_table.shape)
+    lengths = _int32(lengths, "lengths", (R,))
+    P = block_table.shape[1]
+    if scale is None:
+        scale = D ** -0.5
+    out = torch.empty((R, heads, D), dtype=BF16, device=device)
+    lse = torch.empty((R, heads), dtype=torch.float32, device=device) if return_lse else None
+    need = lib.rmoe_paged_attention_workspace_bytes(ctypes.byref(cache), heads, R, P, window)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    with _there(device):
+        _lib.check(lib.rmoe_paged_attention(
+            ctypes.byref(qr), ctypes.byref(cache), block_table.data_ptr(), block_table.stride(0),
+            P, lengths.data_ptr(), R, window, float(scale), out.data_ptr(), _lib.ptr(lse),
+            _lib.ptr(ws), need, _lib.stream_handle(device)))
+    return (out, lse) if return_lse else out
+
+
+def _gate_rows(t: torch.Tensor, name: str, rows: int, heads: int) -> _lib.Gate:
+    if t.dtype != torch.float32 or tuple(t.shape) != (rows, heads):
+        raise ValueError(f"{name} must be float32 [{rows}, {heads}] "
+                         f"(got {t.dtype} {list(t.shape)})")
+    return _lib.Gate(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     log_decay: torch.Tensor, cu_seqlens: torch.Tensor, state: torch.Tensor,
+                     beta: torch.Tensor | None = None, state_index: torch.Tensor | None = None,
+                     scale: float | None = None,
+                     state_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Linear attention with a decay for each head over packed sequences, the
+    delta rule with `beta`: q, k bf16 [N, Hk, Dk], v bf16 [N, Hv, Dv] (value
+    heads share q and k heads in order), log_decay float32 [N, Hv] (any
+    strides: a head's constant expands over the tokens), beta float32 [N, Hv]
+    or None; sequence r is rows cu_seqlens[r] to cu_seqlens[r + 1] (int32 [R +
+    1]).  Per token S <- exp(log_decay) S + k u^T, out = scale S^T q, with u =
+    v, or u = beta (v - (exp(log_decay) S)^T k).  -> bf16 [N, Hv, Dv], zeros in
+    rows of no sequence.
+
+    state float32 [slots, Hv, Dk, Dv] holds the sequences' states, sequence
+    r's at state_index[r] (int [R], each slot at most once; None: r; outside
+    of [0, slots): from zeros, not kept); the final ones go to the same slots
+    of state_out (default: state itself), of which no other slot is touched.
+    Calls of few tokens per sequence run token by token, others in chunks;
+    both hold the state in float32."""
+    lib = _lib.load()
+    device = _one_device(q, k, v, log_decay, cu_seqlens, state, beta, state_index, state_out)
+    q, qr = _heads(q, "q")
+    N, kh, dk = q.shape
+    k, kr = _heads(k, "k", N, kh, dk)
+    v, vr = _heads(v, "v", N)
+    vh, dv = v.shape[1:]
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be [sequences + 1]")
+    R = cu_seqlens.numel() - 1
+    cu_seqlens = _int32(cu_seqlens, "cu_seqlens", (R + 1,))
+    decay = _gate_rows(log_decay, "log_decay", N, vh)
+    gate = None if beta is None else _gate_rows(beta, "beta", N, vh)
+    if state_out is None:
+        state_out = state
+    for t, name in ((state, "state"), (state_out, "state_out")):
+        if (t.dtype != torch.float32 or t.dim() != 4 or tuple(t.shape[1:]) != (vh, dk, dv)
+                or t.shape[0] != state.shape[0] or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 [slots, {vh}, {dk}, {dv}] "
+                             f"(got {t.dtype} {list(t.shape)})")
+    a, b, size = state.data_ptr(), state_out.data_ptr(), 4 * state.numel()
+    if a != b and a < b + size and b < a + size:
+        raise ValueError("state_out must be state or lie apart from it")
+    if state_index is not None:
+        state_index = _int32(state_index, "state_index", (R,))
+    elif state.shape[0] < R:
+        raise ValueError(f"state has {state.shape[0]} slots for {R} sequences")
+    if scale is None:
+        scale = dk ** -0.5
+    if R == 0:
+        return torch.zeros((N, vh, dv), dtype=BF16, device=device)
+    out = torch.empty((N, vh, dv), dtype=BF16, device=device)
+    need = lib.rmoe_linear_attention_workspace_bytes(N, R, kh, vh, dk, int(gate is not None))
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    with _there(device):
+        _lib.check(lib.rmoe_linear_attention(
+            ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr), ctypes.byref(decay),
+            None if gate is None else ctypes.byref(gate), cu_seqlens.data_ptr(), N, R, dk, dv,
+            float(scale), state.data_ptr(), state_out.data_ptr(), _lib.ptr(state_index),
+            state.shape[0], out.data_ptr(), 1, _lib.ptr(ws), need, _lib.stream_handle(device)))
+    return out
+
+
 def stream_read(buf: torch.Tensor, blocks: int, partials: torch.Tensor | None = None):
     lib = _lib.load()
     nbytes = buf.numel() * buf.element_size()

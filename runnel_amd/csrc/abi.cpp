@@ -1275,6 +1275,10 @@ int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_row
   if (q->heads != k->heads || v->heads % k->heads)
     return fail(RMOE_EINVAL, "q and k must share their heads, and v's be a multiple (got %d, %d, %d)",
                 q->heads, k->heads, v->heads);
+  // (the offsets inside a chunk of 64 rows are 32-bit)
+  if (q->row_stride > (1 << 24) || k->row_stride > (1 << 24) || v->row_stride > (1 << 24) ||
+      (int64_t)v->heads * dv > (1 << 24))
+    return fail(RMOE_EINVAL, "rows of more than 2^24 values are not supported");
   if (!log_decay) return fail(RMOE_ENULL, "log_decay: descriptor is NULL");
   if (log_decay->row_stride < 0 || log_decay->head_stride < 0 ||
       (beta && (beta->row_stride < 0 || beta->head_stride < 0)))
@@ -1308,7 +1312,7 @@ int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_row
       return fail(RMOE_EWS, "workspace of %zu bytes needed (got %zu)", (size_t)l.total,
                   workspace_bytes);
     if (!aligned(workspace, 16)) return fail(RMOE_EALIGN, "workspace must be 16-byte aligned");
-    a.workspace = workspace, a.chunks = l.chunks, a.kt_offset = l.kt_offset;
+    a.workspace = workspace, a.chunks = l.chunks, a.key_offset = l.key_offset;
   }
   const hipError_t e = rmoe::launch_linear(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "linear attention launch");

@@ -290,10 +290,10 @@ struct LinearArgs {
   uint16_t* out;              // [tokens, v_heads, dv]
   int clear;                  // rows of no sequence are set to zero
   void* workspace;            // NULL: token by token
-  int64_t chunks, kt_offset;
+  int64_t chunks, key_offset;
 };
 struct LinearLayout {
-  int64_t chunks, kt_offset, total;
+  int64_t chunks, key_offset, total;
 };
 bool linear_in_chunks(int64_t tokens, int requests);
 LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_heads, int dk,

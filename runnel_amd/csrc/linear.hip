@@ -32,6 +32,7 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kLinThreads = 256;
 constexpr float kLeastLogDecay = -1.0e4f;  // exp of it is 0; keeps sums of -inf apart
@@ -171,22 +172,32 @@ __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearAr
 
 // ------------------------------------------------------------------ in chunks
 constexpr int kChunk = 64;
+constexpr int kChunkThreads = 12 * kWave;
 constexpr int kStep = 1024;  // bytes of one operand A of 16 x 32 values, in lane order
 
-// Operand blocks of a wave's 16 rows: columns 0..31 for all four waves, then
-// 32..63 for waves 2 and 3 (the others' are above the diagonal).
-__device__ __forceinline__ int block_of(int wave, int ks) { return ks ? 2 + wave : wave; }
-constexpr int kBlocks = 6;
-
-// Workspace of one (chunk, value head): T's blocks in three pieces, P's in
-// two, then e^G and e^{G_C - G} of its 64 tokens and e^{G_C}.
+// Workspace of one (chunk, value head): the 16 x 16 tiles of T and P on and
+// below the diagonal (tile (w, j) at number w (w + 1) / 2 + j), as operand A in
+// pieces: for each lane its four values of a tile, T's first two pieces and
+// P's two as 16 bytes, T's third as 8; then a line each for the four token
+// waves (e^G and e^{G_C - G} of their tokens) and for the four state waves
+// (e^{G_C}).  Of one (chunk, key head): q and k as operand A.  Every wave that
+// reads these reads whole lines that no other wave of its workgroup does.
+constexpr int kTiles = 10;
 template <bool DELTA>
 struct ChunkData {
-  static constexpr int t = 0;
-  static constexpr int p = DELTA ? kBlocks * 3 * kStep : 0;
-  static constexpr int scal = p + kBlocks * 2 * kStep;
-  static constexpr int bytes = scal + (2 * kChunk + 4) * 4;
+  static constexpr int p = 0;
+  static constexpr int t01 = kTiles * kStep;
+  static constexpr int t2 = DELTA ? 2 * kTiles * kStep : t01;
+  static constexpr int token = DELTA ? t2 + kTiles * kStep / 2 : t01;
+  static constexpr int state = token + 4 * 128;
+  static constexpr int bytes = state + 4 * 128;
 };
+template <int DK>
+struct KeyData {
+  static constexpr int part = DK / 32 * 4 * kStep;
+  static constexpr int q = 0, k = part, bytes = 2 * part;
+};
+__device__ __forceinline__ int tile_of(int w, int j) { return w * (w + 1) / 2 + j; }
 
 // The chunks of sequence r start at number cu[r] / 64 + r, which leaves room
 // for the part chunk that each sequence may end in, and needs no sums.
@@ -241,7 +252,6 @@ __device__ __forceinline__ void lds_barrier() {
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const LinearArgs a) {
   constexpr int KS = DK / 32;
-  constexpr int MT = DK / 64;  // 16-row tiles of the state that a wave keeps
   constexpr int LD = kChunk + 4;
   __shared__ double Gs[kChunk];
   __shared__ float bs[kChunk];
@@ -289,10 +299,10 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
     Gs[lane] = G;
     if constexpr (DELTA)
       bs[lane] = lane < len ? a.beta[(row0 + lane) * a.beta_row + hv * a.beta_head] : 0.0f;
-    float* scal = reinterpret_cast<float*>(ws + ChunkData<DELTA>::scal);
-    scal[lane] = expf((float)G);
-    scal[kChunk + lane] = lane < len ? expf((float)(Gc - G)) : 0.0f;
-    if (lane == 0) scal[2 * kChunk] = expf((float)Gc);
+    float* token = reinterpret_cast<float*>(ws + ChunkData<DELTA>::token) + 32 * g + n;
+    token[0] = expf((float)G);
+    token[16] = lane < len ? expf((float)(Gc - G)) : 0.0f;
+    if (n == 0) *reinterpret_cast<float*>(ws + ChunkData<DELTA>::state + 128 * g) = expf((float)Gc);
   }
 
   // 16 rows of q or k as an operand; rows past the end repeat the last one
@@ -338,44 +348,23 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
     if constexpr (DELTA) *reinterpret_cast<f32x4*>(&As[t * LD + 16 * j + 4 * g]) = kk;
   }
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    if (2 * ks > wave) continue;
-    uint32_t lo[2][2], up[2][2];
-    pieces<2>(pt[2 * ks], lo);
-    pieces<2>(pt[2 * ks + 1], up);
-    uint8_t* dst = ws + ChunkData<DELTA>::p + block_of(wave, ks) * 2 * kStep + lane * 16;
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-      *reinterpret_cast<uint4*>(dst + p * kStep) = make_uint4(lo[p][0], lo[p][1], up[p][0], up[p][1]);
+  for (int j = 0; j < 4; ++j) {
+    if (j > wave) continue;
+    uint32_t w[2][2];
+    pieces<2>(pt[j], w);
+    *reinterpret_cast<uint4*>(ws + ChunkData<DELTA>::p + tile_of(wave, j) * kStep + lane * 16) =
+        make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
   }
 
-  // K^T for the update, once for the value heads that share it: row m of the
-  // wave's tile h is k's dim 32 ks + 8 (m / 4) + 4 h' + m % 4 (ks, h' the tile
-  // number's upper part and lowest bit), the order in which the second
-  // product of the state's own registers needs them
+  // q and k in operand order, once for the value heads that share them: rows
+  // of all heads lie far apart, and a product needs half a line of each
   if (hv % each == 0) {
-    uint8_t* kt = static_cast<uint8_t*>(a.workspace) + a.kt_offset +
-                  (c * a.k_heads + hk) * (int64_t)(8 * MT * kStep);
+    uint8_t* key = static_cast<uint8_t*>(a.workspace) + a.key_offset +
+                   (c * a.k_heads + hk) * (int64_t)KeyData<DK>::bytes + lane * 16;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int tg = wave * MT + mt;
-      const int d = 32 * (tg >> 1) + 8 * (n >> 2) + 4 * (tg & 1) + (n & 3);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          uint32_t x[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = 32 * ks + 16 * ((j + e) >> 2) + 4 * g + ((j + e) & 3);
-            x[e] = a.k[(row0 + (i < len ? i : len - 1)) * a.k_row + hk * a.k_head + d];
-          }
-          w[j >> 1] = x[0] | x[1] << 16;
-        }
-        *reinterpret_cast<uint4*>(kt + ((wave * MT + mt) * 2 + ks) * kStep + lane * 16) =
-            make_uint4(w[0], w[1], w[2], w[3]);
-      }
+    for (int s = 0; s < KS; ++s) {
+      *reinterpret_cast<bf16x8*>(key + KeyData<DK>::q + (4 * s + wave) * kStep) = qf[s];
+      *reinterpret_cast<bf16x8*>(key + KeyData<DK>::k + (4 * s + wave) * kStep) = kf[s];
     }
   }
   if constexpr (!DELTA) return;
@@ -423,248 +412,397 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
   }
   // times B, as operand A in three pieces
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks) {
-    if (2 * ks > wave) continue;
-    uint32_t w[2][3][2];
+  for (int j = 0; j < 4; ++j) {
+    if (j > wave) continue;
+    const int col = 16 * j + 4 * g;
+    f32x4 v = *reinterpret_cast<const f32x4*>(&Ts[t * LD + col]);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (2 * ks + h <= wave) {
-        const int col = 32 * ks + 16 * h + 4 * g;
-        v = *reinterpret_cast<const f32x4*>(&Ts[t * LD + col]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= bs[col + i];
-      }
-      pieces<3>(v, w[h]);
-    }
-    uint8_t* dst = ws + ChunkData<DELTA>::t + block_of(wave, ks) * 3 * kStep + lane * 16;
-#pragma unroll
-    for (int p = 0; p < 3; ++p)
-      *reinterpret_cast<uint4*>(dst + p * kStep) =
-          make_uint4(w[0][p][0], w[0][p][1], w[1][p][0], w[1][p][1]);
+    for (int i = 0; i < 4; ++i) v[i] *= bs[col + i];
+    uint32_t w[3][2];
+    pieces<3>(v, w);
+    const int at = tile_of(wave, j);
+    *reinterpret_cast<uint4*>(ws + ChunkData<DELTA>::t01 + at * kStep + lane * 16) =
+        make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+    *reinterpret_cast<uint2*>(ws + ChunkData<DELTA>::t2 + at * (kStep / 2) + lane * 8) =
+        make_uint2(w[2][0], w[2][1]);
   }
 }
 
+// One (sequence, head, 16 columns of the state) from chunk to chunk, twelve
+// waves, three to a SIMD (one alone waits between its instructions):
+//
+//   - state waves 0 to 3 hold 32 dims of the state each and multiply them, as
+//     they lie in their registers, by those dims of all 64 tokens: an
+//     accumulator's lane holds rows 4 g + i of its column, four of the eight
+//     contraction indices that the same lane needs in operand B;
+//   - token waves 4 to 7 take 16 tokens each, add up the partial K S and make U;
+//   - output waves 8 to 11 take 16 tokens each and make the outputs of the chunk
+//     before.
+//
+// With the delta rule a chunk is a chain of three exchanges through LDS
+// (partial K S, the residual, U) between the first two; what is not in the
+// chain (outputs, q S, turning k, loads) is done by whoever is not in it.
+// Without it U is v, and one exchange is left.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(kLinThreads) void linear_chunk_kernel(const LinearArgs a) {
-  constexpr int KS = DK / 32;
-  constexpr int MT = DK / 64;
-  constexpr int UP = DELTA ? 2 : 1;  // pieces of U in P U (without beta it is v, which is bf16)
-  __shared__ uint4 Sf[3][KS][kWave];
+__global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const LinearArgs a) {
+  constexpr int KS = DK / 32;         // state waves
+  constexpr int SP = DELTA ? 3 : 2;   // pieces of the state that a product takes
+  constexpr int UP = DELTA ? 2 : 1;   // of U in P U (v alone is bf16 as it is)
+  constexpr int BUF = DELTA ? 1 : 2;  // one exchange a chunk: two buffers in turn
+  __shared__ f32x4 Kp[DELTA ? KS : 1][4][kWave];  // partial K S of each 16 tokens
+  __shared__ f32x4 Qp[BUF][KS][4][kWave];         // and Q S
   __shared__ uint4 Rf[DELTA ? 3 : 1][2][kWave];
-  __shared__ uint4 Uf[UP + 3][2][kWave];
+  __shared__ uint4 Uf[BUF][UP + 3][2][kWave];
+  __shared__ uint4 Kt[KS][4][kWave];              // a state wave's dims of k, to be transposed
 
   // the column tiles of a head on one XCD, whose L2 holds the head's chunk
   const int tiles = a.dv / 16;
   const int64_t heads = (int64_t)a.requests * a.v_heads;
-  const int64_t b = blockIdx.x;
-  const int64_t per_xcd = (heads + 7) / 8 * tiles;
-  const int64_t in_xcd = b >> 3;
-  const int64_t head = (in_xcd / tiles) * 8 + (b & 7);
-  if (in_xcd >= per_xcd || head >= heads) return;
+  const int64_t in_xcd = blockIdx.x >> 3;
+  const int64_t head = in_xcd / tiles * 8 + (blockIdx.x & 7);
+  if (head >= heads) return;
   const int tile = (int)(in_xcd % tiles);
   const int r = (int)(head / a.v_heads), hv = (int)(head - (int64_t)r * a.v_heads);
   const int hk = hv / (a.v_heads / a.k_heads);
   const Seq sq = seq_of(a, r);
   const int64_t slot = slot_of(a, r);
 
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w4 = wave & 3;  // its dims 32 w4 .. or its tokens 16 w4 ..
   const int n = lane & 15, g = lane >> 4;
   const int col = tile * 16 + n;
-
-  // state: tile tg = wave MT + mt, lane (g, n): dims 32 (tg / 2) + 8 g +
-  // 4 (tg % 2) + i of column n
-  f32x4 S[MT];
-  int64_t at[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int tg = wave * MT + mt;
-    const int d = 32 * (tg >> 1) + 8 * g + 4 * (tg & 1);
-    at[mt] = ((slot * a.v_heads + hv) * DK + d) * a.dv + col;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) S[mt][i] = slot >= 0 ? a.state[at[mt] + (int64_t)i * a.dv] : 0.0f;
-  }
-
   const int chunks = (sq.len + kChunk - 1) / kChunk;
   const int64_t c0 = chunk_base(a, r);
-  const uint8_t* ws0 = static_cast<const uint8_t*>(a.workspace) +
-                       (c0 * a.v_heads + hv) * (int64_t)ChunkData<DELTA>::bytes;
+  const char* ws0 = static_cast<const char*>(a.workspace) +
+                    (c0 * a.v_heads + hv) * (int64_t)ChunkData<DELTA>::bytes;
   const int64_t ws_step = (int64_t)a.v_heads * ChunkData<DELTA>::bytes;
-  const uint8_t* kt0 = static_cast<const uint8_t*>(a.workspace) + a.kt_offset +
-                       (c0 * a.k_heads + hk) * (int64_t)(8 * MT * kStep);
-  const int64_t kt_step = (int64_t)a.k_heads * (8 * MT * kStep);
-  const bool two = wave >= 2;  // blocks of the second 32 columns
+  const uint32_t l16 = lane * 16;
+  // Operands are loaded two chunks ahead, into two sets used in turn, by each
+  // kind of wave while the chain is with the other kind; past the end the last
+  // chunk's are loaded again, which needs no branch.
+  auto clamped = [&](int c) { return c < chunks ? c : chunks - 1; };
 
-  uint4 kf[KS], qf[KS], ktf[MT][2], tf[DELTA ? 3 : 1][2], pf[2][2];
-  uint32_t vv[4];
-  float eG[4], dec[4], eC;
-  auto load_kq = [&](int c) {
-    if (c >= chunks) return;
-    const int i = c * kChunk + 16 * wave + n;
-    const int64_t row = sq.begin + (i < sq.len ? i : sq.len - 1);
-    const uint16_t* kp = a.k + row * a.k_row + hk * a.k_head + 8 * g;
-    const uint16_t* qp = a.q + row * a.q_row + hk * a.q_head + 8 * g;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if constexpr (DELTA) kf[s] = load16(kp + 32 * s);
-      qf[s] = load16(qp + 32 * s);
-    }
-  };
-  auto load_v = [&](int c) {
-    if (c >= chunks) return;
-    const float* scal = reinterpret_cast<const float*>(ws0 + c * ws_step + ChunkData<DELTA>::scal);
-    const int i0 = 16 * wave + 4 * g;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = c * kChunk + i0 + i;
-      const int64_t row = sq.begin + (j < sq.len ? j : sq.len - 1);
-      vv[i] = a.v[row * a.v_row + hv * a.v_head + col];
-    }
-    const f32x4 e = *reinterpret_cast<const f32x4*>(scal + i0);
-    const f32x4 d = *reinterpret_cast<const f32x4*>(scal + kChunk + i0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) eG[i] = e[i], dec[i] = d[i];
-    eC = scal[2 * kChunk];
-  };
-  auto load_t = [&](int c) {
-    if (!DELTA || c >= chunks) return;
-    const uint8_t* p = ws0 + c * ws_step + ChunkData<DELTA>::t + lane * 16;
-#pragma unroll
-    for (int i = 0; i < (DELTA ? 3 : 0); ++i) {
-      tf[i][0] = load16(p + (block_of(wave, 0) * 3 + i) * kStep);
-      if (two) tf[i][1] = load16(p + (block_of(wave, 1) * 3 + i) * kStep);
-    }
-  };
-  auto load_p = [&](int c) {
-    if (c >= chunks) return;
-    const uint8_t* p = ws0 + c * ws_step + ChunkData<DELTA>::p + lane * 16;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      pf[i][0] = load16(p + (block_of(wave, 0) * 2 + i) * kStep);
-      if (two) pf[i][1] = load16(p + (block_of(wave, 1) * 2 + i) * kStep);
-    }
-    const uint8_t* k = kt0 + c * kt_step + lane * 16;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) ktf[mt][ks] = load16(k + ((wave * MT + mt) * 2 + ks) * kStep);
-  };
-  load_kq(0);
-  load_v(0);
-  load_t(0);
-  load_p(0);
-
-  for (int c = 0; c < chunks; ++c) {
-    // the state in three pieces, as operand B of the wave's dims
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int tg = wave * MT + mt;
-      uint32_t w[3][2];
-      pieces<3>(S[mt], w);
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        reinterpret_cast<uint2*>(&Sf[p][tg >> 1][lane])[tg & 1] = make_uint2(w[p][0], w[p][1]);
-    }
-    lds_barrier();
-    f32x4 ksum[3], qsum[2];
-#pragma unroll
-    for (int p = 0; p < 3; ++p) ksum[p] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    qsum[0] = qsum[1] = ksum[0];
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        if (!DELTA && p == 2) continue;
-        const bf16x8 f = frag(Sf[p][s][lane]);
-        if constexpr (DELTA) ksum[p] = mfma(frag(kf[s]), f, ksum[p]);
-        if (p < 2) qsum[p] = mfma(frag(qf[s]), f, qsum[p]);
+  if (wave < 4) {
+    // -------------------------------------------------------- state waves
+    if (w4 >= KS) {  // with 64 dims there are two
+      for (int c = 0; c < chunks; ++c) {
+        lds_barrier();
+        if constexpr (DELTA) {
+          lds_barrier();
+          lds_barrier();
+        }
       }
-    load_kq(c + 1);
-
-    f32x4 u;
-    if constexpr (DELTA) {
+      return;
+    }
+    // lane (g, n) of tile h: dims 32 w4 + 8 g + 4 h + i of column n
+    f32x4 S[2];
+    const int64_t at = ((slot * a.v_heads + hv) * DK + 32 * w4 + 8 * g) * a.dv + col;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        u[i] = bf16_to_f32(vv[i]) - eG[i] * (ksum[0][i] + (ksum[1][i] + ksum[2][i]));
+        S[h][i] = slot >= 0 ? a.state[at + (int64_t)(4 * h + i) * a.dv] : 0.0f;
+
+    const char* key0 = static_cast<const char*>(a.workspace) + a.key_offset +
+                       (c0 * a.k_heads + hk) * (int64_t)KeyData<DK>::bytes + w4 * 4 * kStep;
+    const int64_t key_step = (int64_t)a.k_heads * KeyData<DK>::bytes;
+    struct Loads {
+      uint4 k[4], q[4];
+      float eC;
+    };
+    // the wave's dims of 64 tokens of k and of q
+    auto load = [&](int c, Loads& x) {
+      c = clamped(c);
+      const char* k = key0 + c * key_step;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x.k[t] = load16(k + KeyData<DK>::k + t * kStep + l16);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x.q[t] = load16(k + KeyData<DK>::q + t * kStep + l16);
+      x.eC = *reinterpret_cast<const float*>(ws0 + c * ws_step + ChunkData<DELTA>::state +
+                                             128 * w4 + 4 * (uint32_t)(lane >> 6));
+    };
+    // K^T as operand A: the wave's own dims, turned in LDS.  The transposing
+    // read gives lane m of 16 column m of the 4 rows of 16 values that the 16
+    // lanes' addresses (4 values each) name: rows are tokens 4 g + i, columns
+    // dims 8 (m / 4) + 4 h + m % 4, the order of the state's registers.
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+    const int turned = ((n & 3) * 16 + 4 * g + (n >> 2)) * 8;  // in 2-byte values
+    auto transpose = [&](const Loads& x, bf16x8(&kt)[2][2]) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) Kt[w4][t][lane] = x.k[t];
+      uint16_t* base = reinterpret_cast<uint16_t*>(&Kt[w4][0][0]) + turned;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          union {
+            s16x4 half[2];
+            bf16x8 v;
+          } u;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            u.half[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4)(base + (2 * ks + e) * (kStep / 2) + 4 * h));
+          kt[h][ks] = u.v;
+        }
+    };
+    auto step = [&](int c, Loads& now) {
+      const int b = DELTA ? 0 : c & 1;
+      uint32_t lo[SP][2], up[SP][2];
+      pieces<SP>(S[0], lo);
+      pieces<SP>(S[1], up);
+      bf16x8 sf[SP];
+#pragma unroll
+      for (int p = 0; p < SP; ++p) {
+        const uint32_t w[4] = {lo[p][0], lo[p][1], up[p][0], up[p][1]};
+        sf[p] = frag(w);
+      }
+      if constexpr (DELTA) {
+        f32x4 x[4] = {};
+#pragma unroll
+        for (int p = SP - 1; p >= 0; --p)  // from the least up
+#pragma unroll
+          for (int t = 0; t < 4; ++t) x[t] = mfma(frag(now.k[t]), sf[p], x[t]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) Kp[w4][t][lane] = x[t];
+        lds_barrier();
+      }
+      bf16x8 kt[2][2];
+      transpose(now, kt);
+      {
+        f32x4 x[4] = {};
+#pragma unroll
+        for (int p = 1; p >= 0; --p)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) x[t] = mfma(frag(now.q[t]), sf[p], x[t]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) Qp[b][w4][t][lane] = x[t];
+      }
+      const float eC = now.eC;
+      load(c + 2, now);
+      lds_barrier();
+      if constexpr (DELTA) lds_barrier();
+      uint4 uf[3][2];
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) uf[p][ks] = Uf[b][UP + p][ks][lane];
+      issue_fence();
+      f32x4 y[2][2] = {};
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            y[h][ks] = mfma(kt[h][ks], frag(uf[p][ks]), y[h][ks]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) S[h] = eC * S[h] + (y[h][0] + y[h][1]);
+    };
+    if (chunks > 0) {
+      Loads even, odd;
+      load(0, even);
+      load(1, odd);
+      int c = 0;
+      for (; c + 1 < chunks; c += 2) {
+        step(c, even);
+        step(c + 1, odd);
+      }
+      if (c < chunks) step(c, even);
+    }
+    if (slot < 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a.state_out[at + (int64_t)(4 * h + i) * a.dv] = S[h][i];
+    return;
+  }
+
+  if (chunks == 0) return;
+  const bool two = w4 >= 2;  // tiles of the second 32 columns
+  const int tile0 = tile_of(w4, 0);
+  const int i0 = 16 * w4 + 4 * g;
+  auto load_scalars = [&](int c, int which) {
+    return *reinterpret_cast<const f32x4*>(ws0 + c * ws_step + ChunkData<DELTA>::token +
+                                           128 * w4 + 64 * which + 16 * (uint32_t)g);
+  };
+
+  if (wave >= 8) {
+    // ------------------------------------------------------- output waves
+    u32x4 p[4];
+    f32x4 eG, qs;
+    uint4 u[UP][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = (u32x4){0, 0, 0, 0};  // above the diagonal: stay zero
+    auto load = [&](int c) {
+      c = clamped(c);
+      const char* m = ws0 + c * ws_step + ChunkData<DELTA>::p + tile0 * kStep;
+      eG = load_scalars(c, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= w4) p[j] = *reinterpret_cast<const u32x4*>(m + j * kStep + l16);
+    };
+    auto take = [&](int b) {
+      f32x4 q[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] = Qp[b][s][w4][lane];
+#pragma unroll
+      for (int e = 0; e < UP; ++e) u[e][0] = Uf[b][e][0][lane], u[e][1] = Uf[b][e][1][lane];
+      qs = q[0] + q[1];
+      if constexpr (KS == 4) qs += q[2] + q[3];
+    };
+    // scale (e^G q S + P U)
+    const int64_t o_row = (int64_t)a.v_heads * a.dv;
+    auto finish = [&](int c) {
+      f32x4 o0 = {0.0f, 0.0f, 0.0f, 0.0f}, o1 = o0, o2 = o0;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks && !two) continue;
+        const u32x4 l = p[2 * ks], r = p[2 * ks + 1];
+        const bf16x8 p0 = frag(make_uint4(l.x, l.y, r.x, r.y));
+        o0 = mfma(p0, frag(u[0][ks]), o0);
+        o1 = mfma(frag(make_uint4(l.z, l.w, r.z, r.w)), frag(u[0][ks]), o1);
+        if constexpr (DELTA) o2 = mfma(p0, frag(u[UP - 1][ks]), o2);
+      }
+      const f32x4 o = a.scale * (eG * qs + (o0 + (o1 + o2)));
+      char* base = reinterpret_cast<char*>(
+          a.out + (sq.begin + (int64_t)c * kChunk) * o_row + (int64_t)hv * a.dv);
+      const int left = sq.len - c * kChunk;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i0 + i < left)
+          *reinterpret_cast<uint16_t*>(
+              base + ((uint32_t)(i0 + i) * ((uint32_t)o_row * 2u) + 2u * (uint32_t)col)) =
+              (uint16_t)f32_to_bf16(o[i]);
+      load(c + 1);
+    };
+    load(0);
+    for (int c = 0; c < chunks; ++c) {
+      if constexpr (DELTA) {
+        lds_barrier();
+        if (c > 0) finish(c - 1);
+        lds_barrier();
+        lds_barrier();
+        take(0);
+      } else {
+        lds_barrier();
+        take(c & 1);
+        finish(c);
+      }
+    }
+    if constexpr (DELTA) finish(chunks - 1);
+    return;
+  }
+
+  // ---------------------------------------------------------- token waves
+  struct Loads {
+    u32x4 t01[DELTA ? 4 : 1];
+    u32x2 t2[DELTA ? 4 : 1];
+    uint16_t v[4];
+    f32x4 eG, dec;
+  };
+  auto load = [&](int c, Loads& x) {
+    c = clamped(c);
+    const char* m = ws0 + c * ws_step;
+    if constexpr (DELTA) x.eG = load_scalars(c, 0);
+    x.dec = load_scalars(c, 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j > w4) continue;
+      if constexpr (DELTA) {
+        x.t01[j] = *reinterpret_cast<const u32x4*>(m + ChunkData<DELTA>::t01 + (tile0 + j) * kStep + l16);
+        x.t2[j] = *reinterpret_cast<const u32x2*>(m + ChunkData<DELTA>::t2 +
+                                                  (tile0 + j) * (kStep / 2) + l16 / 2);
+      }
+    }
+    const int last = sq.len - c * kChunk - 1;
+    const char* base = reinterpret_cast<const char*>(
+        a.v + (sq.begin + (int64_t)c * kChunk) * a.v_row + hv * a.v_head);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x.v[e] = *reinterpret_cast<const uint16_t*>(
+          base + ((uint32_t)min(i0 + e, last) * ((uint32_t)a.v_row * 2u) + 2u * (uint32_t)col));
+  };
+  auto put_u = [&](int b, const f32x4 u, const f32x4 dec) {
+    uint32_t w[UP][2], y[3][2];
+    pieces<3>(dec * u, y);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      reinterpret_cast<uint2*>(&Uf[b][UP + p][w4 >> 1][lane])[w4 & 1] = make_uint2(y[p][0], y[p][1]);
+    pieces<UP>(u, w);
+#pragma unroll
+    for (int p = 0; p < UP; ++p)
+      reinterpret_cast<uint2*>(&Uf[b][p][w4 >> 1][lane])[w4 & 1] = make_uint2(w[p][0], w[p][1]);
+  };
+  auto step = [&](int c, Loads& x) {
+    const int b = DELTA ? 0 : c & 1;
+    f32x4 u;
+    if constexpr (DELTA) {
+      lds_barrier();
+      f32x4 k[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) k[s] = Kp[s][w4][lane];
+      f32x4 ks = k[0] + k[1];
+      if constexpr (KS == 4) ks += k[2] + k[3];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = bf16_to_f32(x.v[i]) - x.eG[i] * ks[i];
       uint32_t w[3][2];
       pieces<3>(u, w);
 #pragma unroll
       for (int p = 0; p < 3; ++p)
-        reinterpret_cast<uint2*>(&Rf[p][wave >> 1][lane])[wave & 1] = make_uint2(w[p][0], w[p][1]);
+        reinterpret_cast<uint2*>(&Rf[p][w4 >> 1][lane])[w4 & 1] = make_uint2(w[p][0], w[p][1]);
       lds_barrier();
-      f32x4 big = {0.0f, 0.0f, 0.0f, 0.0f}, small = big, least = big;
+      uint4 rf[3][2];
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        if (ks && !two) continue;
-        const bf16x8 r0 = frag(Rf[0][ks][lane]), r1 = frag(Rf[1][ks][lane]),
-                     r2 = frag(Rf[2][ks][lane]);
-        const bf16x8 t0 = frag(tf[0][ks]), t1 = frag(tf[1][ks]), t2 = frag(tf[2][ks]);
-        big = mfma(t0, r0, big);
-        small = mfma(t0, r1, small);
-        least = mfma(t0, r2, least);
-        small = mfma(t1, r0, small);
-        least = mfma(t1, r1, least);
-        least = mfma(t2, r0, least);
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) rf[p][s] = Rf[p][s][lane];
+      issue_fence();
+      // six chains of one or two products; the sum goes from the least up
+      f32x4 y[6] = {};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s && !two) continue;
+        const u32x4 l = x.t01[2 * s], r = x.t01[2 * s + 1];
+        const u32x2 l2 = x.t2[2 * s], r2 = x.t2[2 * s + 1];
+        const bf16x8 t0 = frag(make_uint4(l.x, l.y, r.x, r.y));
+        const bf16x8 t1 = frag(make_uint4(l.z, l.w, r.z, r.w));
+        const bf16x8 t2 = frag(make_uint4(l2.x, l2.y, r2.x, r2.y));
+        y[0] = mfma(t0, frag(rf[0][s]), y[0]);
+        y[1] = mfma(t0, frag(rf[1][s]), y[1]);
+        y[2] = mfma(t1, frag(rf[0][s]), y[2]);
+        y[3] = mfma(t0, frag(rf[2][s]), y[3]);
+        y[4] = mfma(t1, frag(rf[1][s]), y[4]);
+        y[5] = mfma(t2, frag(rf[0][s]), y[5]);
       }
-      u = big + (small + least);
-      load_t(c + 1);
+      u = y[0] + ((y[1] + y[2]) + (y[3] + (y[4] + y[5])));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = bf16_to_f32(vv[i]);
+      for (int i = 0; i < 4; ++i) u[i] = bf16_to_f32(x.v[i]);
     }
-    {
-      uint32_t w[UP][2], x[3][2];
-      pieces<UP>(u, w);
-      f32x4 d;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = dec[i] * u[i];
-      pieces<3>(d, x);
-#pragma unroll
-      for (int p = 0; p < UP; ++p)
-        reinterpret_cast<uint2*>(&Uf[p][wave >> 1][lane])[wave & 1] = make_uint2(w[p][0], w[p][1]);
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        reinterpret_cast<uint2*>(&Uf[UP + p][wave >> 1][lane])[wave & 1] =
-            make_uint2(x[p][0], x[p][1]);
-    }
+    put_u(b, u, x.dec);
     lds_barrier();
-    f32x4 o0 = {0.0f, 0.0f, 0.0f, 0.0f}, o1 = o0;
+    load(c + 2, x);
+  };
+  Loads even, odd;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks && !two) continue;
-      const bf16x8 u0 = frag(Uf[0][ks][lane]);
-      o0 = mfma(frag(pf[0][ks]), u0, o0);
-      o1 = mfma(frag(pf[1][ks]), u0, o1);
-      if constexpr (DELTA) o1 = mfma(frag(pf[0][ks]), frag(Uf[1][ks][lane]), o1);
+  for (int j = 0; j < 4; ++j) {  // the tiles above the diagonal stay zero
+    if constexpr (DELTA) {
+      even.t01[j] = odd.t01[j] = (u32x4){0, 0, 0, 0};
+      even.t2[j] = odd.t2[j] = (u32x2){0, 0};
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0, s2 = s0;
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const bf16x8 k = frag(ktf[mt][ks]);
-        s0 = mfma(k, frag(Uf[UP][ks][lane]), s0);
-        s1 = mfma(k, frag(Uf[UP + 1][ks][lane]), s1);
-        s2 = mfma(k, frag(Uf[UP + 2][ks][lane]), s2);
-      }
-      S[mt] = eC * S[mt] + (s0 + (s1 + s2));
-    }
-    load_p(c + 1);
-    const int i0 = c * kChunk + 16 * wave + 4 * g;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float o = a.scale * (eG[i] * (qsum[0][i] + qsum[1][i]) + (o0[i] + o1[i]));
-      if (i0 + i < sq.len)
-        a.out[((sq.begin + i0 + i) * a.v_heads + hv) * a.dv + col] = (uint16_t)f32_to_bf16(o);
-    }
-    load_v(c + 1);
   }
-  if (slot < 0) return;
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a.state_out[at[mt] + (int64_t)i * a.dv] = S[mt][i];
+  load(0, even);
+  load(1, odd);
+  int c = 0;
+  for (; c + 1 < chunks; c += 2) {
+    step(c, even);
+    step(c + 1, odd);
+  }
+  if (c < chunks) step(c, even);
 }
 
 template <int DK, bool DELTA>
@@ -682,7 +820,7 @@ hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   const int64_t heads = (int64_t)a.requests * a.v_heads;
   linear_chunk_kernel<DK, DELTA>
-      <<<(unsigned)((heads + 7) / 8 * 8 * tiles), kLinThreads, 0, s>>>(a);
+      <<<(unsigned)((heads + 7) / 8 * 8 * tiles), kChunkThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -694,9 +832,10 @@ LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_head
                            bool delta) {
   LinearLayout l;
   l.chunks = tokens / kChunk + requests;
-  l.kt_offset = l.chunks * v_heads *
-                (int64_t)(delta ? ChunkData<true>::bytes : ChunkData<false>::bytes);
-  l.total = l.kt_offset + l.chunks * k_heads * (int64_t)(8 * (dk / 64) * kStep);
+  l.key_offset = l.chunks * v_heads *
+                 (int64_t)(delta ? ChunkData<true>::bytes : ChunkData<false>::bytes);
+  l.total = l.key_offset + l.chunks * k_heads *
+                               (int64_t)(dk == 64 ? KeyData<64>::bytes : KeyData<128>::bytes);
   return l;
 }
 

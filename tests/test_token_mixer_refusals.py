@@ -137,7 +137,8 @@ def test_linear_refusals():
     for bad in (dict(n=-1), dict(r=0), dict(dk=96), dict(dk=256), dict(dv=8), dict(dv=24), dict(dv=1040),
                 dict(q=rows(heads=2)), dict(v=rows(heads=6)), dict(scale=float("nan")), dict(slots=-1),
                 dict(g=_lib.Gate(FAKE, -1, 1)), dict(b=_lib.Gate(FAKE, 1, -1)), dict(n=1 << 30, r=1),
-                dict(r=1 << 30)):
+                dict(r=1 << 30), dict(k=rows(row=1 << 25)), dict(v=rows(row=1 << 25)),
+                dict(v=rows(heads=65536), dv=512)):
         assert call(**bad) == _lib.RMOE_EINVAL, bad
     for bad in (dict(g=None), dict(cu=None), dict(st=None), dict(so=None), dict(out=None), dict(q=rows(x=None)),
                 dict(b=_lib.Gate(None, 1, 1))):

@@ -1304,8 +1304,9 @@ int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_row
   a.out = out, a.clear = clear_uncovered != 0 && tokens > 0;
   const rmoe::LinearLayout l =
       rmoe::linear_layout(tokens, requests, a.k_heads, a.v_heads, dk, a.delta);
-  const int64_t tiles = (int64_t)requests * a.v_heads * (dv / 16);
-  if (tiles + 8 * 64 > kMaxGroups || l.chunks * a.v_heads + 64 > kMaxGroups)
+  // workgroups of 768 threads, for whole eights of key heads
+  const int64_t tiles = ((int64_t)requests * a.k_heads + 8) * (a.v_heads / a.k_heads) * (dv / 16);
+  if (tiles > kMaxGroups / 3 || l.chunks * a.v_heads + 64 > kMaxGroups)
     return fail(RMOE_EINVAL, "too many sequences, tokens or heads for one call");
   if (rmoe::linear_in_chunks(tokens, requests)) {
     if (!workspace || workspace_bytes < (size_t)l.total)

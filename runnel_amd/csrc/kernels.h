@@ -291,6 +291,7 @@ struct LinearArgs {
   int clear;                  // rows of no sequence are set to zero
   void* workspace;            // NULL: token by token
   int64_t chunks, key_offset;
+  int span;                   // value heads side by side on an XCD (set by launch_linear)
 };
 struct LinearLayout {
   int64_t chunks, key_offset, total;

@@ -249,14 +249,22 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// Everything of a chunk that no state goes into, a workgroup per (chunk,
+// value head), 16 tokens a wave.  Bound by the latency of its steps, so it
+// keeps few registers and 30 KB of LDS: five workgroups a compute unit.  Each
+// wave loads its own 16 rows of k and takes the others' from LDS (from memory
+// each tile was a wait of its own); exponentials are of sums kept in base 2.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const LinearArgs a) {
+__global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const LinearArgs a) {
   constexpr int KS = DK / 32;
-  constexpr int LD = kChunk + 4;
+  constexpr int LD = 20;              // row of a 16 x 16 tile in LDS
+  constexpr int TILE = 16 * LD;
   __shared__ double Gs[kChunk];
-  __shared__ float bs[kChunk];
-  __shared__ float As[DELTA ? kChunk * LD : 1];
-  __shared__ float Ts[DELTA ? kChunk * LD : 1];
+  __shared__ __align__(16) float bs[kChunk];
+  __shared__ __align__(16) float As[DELTA ? kTiles * TILE : 4];
+  // k as operand rows, then (with every wave past that) T
+  constexpr int SHARED = KS * 4 * kWave * 4;
+  __shared__ __align__(16) float Ts[SHARED > kTiles * TILE ? SHARED : kTiles * TILE];
 
   const int64_t blocks = a.chunks * a.v_heads;
   if (blockIdx.x >= blocks) {
@@ -284,9 +292,24 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
+  const int t = 16 * wave + n;  // the lane's token
 
-  // running sums of the log decays, one token a lane
-  double G = lane < len ? (double)log_decay(a, row0 + lane, hv) : 0.0;
+  // 16 rows of k and of q as operands; rows past the end repeat the last one
+  uint4 kf[KS], qf[KS];
+  {
+    const int64_t row = row0 + (t < len ? t : len - 1);
+    const uint16_t* kp = a.k + row * a.k_row + hk * a.k_head + 8 * g;
+    const uint16_t* qp = a.q + row * a.q_row + hk * a.q_head + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kf[s] = load16(kp + 32 * s);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = load16(qp + 32 * s);
+  }
+  // running sums of the log decays in base 2, one token a lane
+  constexpr double kLog2e = 1.44269504088896340736;
+  double G = lane < len ? (double)log_decay(a, row0 + lane, hv) * kLog2e : 0.0;
+  float beta = 0.0f;
+  if (DELTA && lane < len) beta = a.beta[(row0 + lane) * a.beta_row + hv * a.beta_head];
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
     const double up = __shfl_up(G, d, kWave);
@@ -297,63 +320,47 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
                 (c * a.v_heads + hv) * (int64_t)ChunkData<DELTA>::bytes;
   if (wave == 0) {
     Gs[lane] = G;
-    if constexpr (DELTA)
-      bs[lane] = lane < len ? a.beta[(row0 + lane) * a.beta_row + hv * a.beta_head] : 0.0f;
+    if constexpr (DELTA) bs[lane] = beta;
     float* token = reinterpret_cast<float*>(ws + ChunkData<DELTA>::token) + 32 * g + n;
-    token[0] = expf((float)G);
-    token[16] = lane < len ? expf((float)(Gc - G)) : 0.0f;
-    if (n == 0) *reinterpret_cast<float*>(ws + ChunkData<DELTA>::state + 128 * g) = expf((float)Gc);
+    token[0] = __builtin_amdgcn_exp2f((float)G);
+    token[16] = lane < len ? __builtin_amdgcn_exp2f((float)(Gc - G)) : 0.0f;
+    if (n == 0)
+      *reinterpret_cast<float*>(ws + ChunkData<DELTA>::state + 128 * g) =
+          __builtin_amdgcn_exp2f((float)Gc);
   }
-
-  // 16 rows of q or k as an operand; rows past the end repeat the last one
-  auto rows16 = [&](const uint16_t* x, int64_t row_stride, int64_t head_stride, int tile,
-                    bf16x8(&f)[KS]) {
-    const int i = 16 * tile + n;
-    const uint16_t* p = x + (row0 + (i < len ? i : len - 1)) * row_stride + hk * head_stride + 8 * g;
+  uint4* Ks = reinterpret_cast<uint4*>(Ts);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) f[s] = frag(load16(p + 32 * s));
-  };
-  bf16x8 kf[KS], qf[KS];
-  rows16(a.k, a.k_row, a.k_head, wave, kf);
-  rows16(a.q, a.q_row, a.q_head, wave, qf);
+  for (int s = 0; s < KS; ++s) Ks[(s * 4 + wave) * kWave + lane] = kf[s];
   __syncthreads();
 
   // K_j K_w^T and K_j Q_w^T, tile j of the columns against the wave's own
   // rows: lane (g, n) gets row t = 16 w + n, columns 16 j + 4 g + i, which is
   // operand A's order (contraction index 8 g + 4 (j & 1) + i)
-  const int t = 16 * wave + n;
   const double Gt = Gs[t];
   const float bt = DELTA ? bs[t] : 0.0f;
-  f32x4 pt[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    pt[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     if (j > wave) continue;
-    bf16x8 kj[KS];
-    rows16(a.k, a.k_row, a.k_head, j, kj);
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      if constexpr (DELTA) kk = mfma(kj[s], kf[s], kk);
-      qk = mfma(kj[s], qf[s], qk);
+      const bf16x8 kj = frag(Ks[(s * 4 + j) * kWave + lane]);
+      if constexpr (DELTA) kk = mfma(kj, frag(kf[s]), kk);
+      qk = mfma(kj, frag(qf[s]), qk);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int m = 16 * j + 4 * g + i;
-      const float e = m <= t && t < len ? expf((float)(Gt - Gs[m])) : 0.0f;
-      qk[i] = m <= t && t < len ? qk[i] * e : 0.0f;
-      kk[i] = m < t && t < len ? bt * (kk[i] * e) : 0.0f;
+      const bool in = m <= t && t < len;
+      const float e = __builtin_amdgcn_exp2f((float)(Gt - Gs[m]));
+      qk[i] = in ? qk[i] * e : 0.0f;
+      kk[i] = in && m < t ? bt * (kk[i] * e) : 0.0f;
     }
-    pt[j] = qk;
-    if constexpr (DELTA) *reinterpret_cast<f32x4*>(&As[t * LD + 16 * j + 4 * g]) = kk;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j > wave) continue;
     uint32_t w[2][2];
-    pieces<2>(pt[j], w);
+    pieces<2>(qk, w);
     *reinterpret_cast<uint4*>(ws + ChunkData<DELTA>::p + tile_of(wave, j) * kStep + lane * 16) =
         make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+    if constexpr (DELTA) *reinterpret_cast<f32x4*>(&As[tile_of(wave, j) * TILE + n * LD + 4 * g]) = kk;
   }
 
   // q and k in operand order, once for the value heads that share them: rows
@@ -363,29 +370,30 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
                    (c * a.k_heads + hk) * (int64_t)KeyData<DK>::bytes + lane * 16;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      *reinterpret_cast<bf16x8*>(key + KeyData<DK>::q + (4 * s + wave) * kStep) = qf[s];
-      *reinterpret_cast<bf16x8*>(key + KeyData<DK>::k + (4 * s + wave) * kStep) = kf[s];
+      *reinterpret_cast<uint4*>(key + KeyData<DK>::q + (4 * s + wave) * kStep) = qf[s];
+      *reinterpret_cast<uint4*>(key + KeyData<DK>::k + (4 * s + wave) * kStep) = kf[s];
     }
   }
   if constexpr (!DELTA) return;
 
-  // T = (I + A)^-1: the four diagonal blocks by substitution, a column a
-  // lane; then T_ij = -T_ii sum_k A_ik T_kj, one diagonal of blocks after
-  // the other, on the fp32 matrix instruction.
+  // T = (I + A)^-1: the four diagonal tiles by substitution, a column a lane;
+  // then T_ij = -T_ii sum_k A_ik T_kj, one diagonal of tiles after the other,
+  // on the fp32 matrix instruction.
   __syncthreads();
   {
-    const int d0 = 16 * wave;
+    const float* d = &As[tile_of(wave, wave) * TILE];
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float acc = i == n ? 1.0f : 0.0f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) acc = fmaf(-As[(d0 + i) * LD + d0 + j], x[j], acc);
+      for (int j = 0; j < i; ++j) acc = fmaf(-d[i * LD + j], x[j], acc);
       x[i] = acc;
     }
     if (g == 0) {
+      float* o = &Ts[tile_of(wave, wave) * TILE];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) Ts[(d0 + i) * LD + d0 + n] = x[i];
+      for (int i = 0; i < 16; ++i) o[i * LD + n] = x[i];
     }
   }
   __syncthreads();
@@ -394,19 +402,22 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
     if (wave + d < 4) {
       const int bi = wave + d, bj = wave;
       f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int k = bj; k < bi; ++k) {
-        const f32x4 av = *reinterpret_cast<const f32x4*>(&As[(16 * bi + n) * LD + 16 * k + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < d; ++e) {
+        const int k = bj + e;
+        const f32x4 av = *reinterpret_cast<const f32x4*>(&As[tile_of(bi, k) * TILE + n * LD + 4 * g]);
+        const float* tk = &Ts[tile_of(k, bj) * TILE + 4 * g * LD + n];
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          x = __builtin_amdgcn_mfma_f32_16x16x4f32(
-              av[s], Ts[(16 * k + 4 * g + s) * LD + 16 * bj + n], x, 0, 0, 0);
+          x = __builtin_amdgcn_mfma_f32_16x16x4f32(av[s], tk[s * LD], x, 0, 0, 0);
       }
-      const f32x4 dv = *reinterpret_cast<const f32x4*>(&Ts[(16 * bi + n) * LD + 16 * bi + 4 * g]);
+      const f32x4 dv = *reinterpret_cast<const f32x4*>(&Ts[tile_of(bi, bi) * TILE + n * LD + 4 * g]);
       f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_16x16x4f32(-dv[s], x[s], y, 0, 0, 0);
+      float* o = &Ts[tile_of(bi, bj) * TILE + 4 * g * LD + n];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) Ts[(16 * bi + 4 * g + s) * LD + 16 * bj + n] = y[s];
+      for (int s = 0; s < 4; ++s) o[s * LD] = y[s];
     }
     __syncthreads();
   }
@@ -414,13 +425,11 @@ __global__ __launch_bounds__(kLinThreads) void linear_prepare_kernel(const Linea
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (j > wave) continue;
-    const int col = 16 * j + 4 * g;
-    f32x4 v = *reinterpret_cast<const f32x4*>(&Ts[t * LD + col]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= bs[col + i];
+    const int at = tile_of(wave, j);
+    f32x4 v = *reinterpret_cast<const f32x4*>(&Ts[at * TILE + n * LD + 4 * g]);
+    v *= *reinterpret_cast<const f32x4*>(&bs[16 * j + 4 * g]);
     uint32_t w[3][2];
     pieces<3>(v, w);
-    const int at = tile_of(wave, j);
     *reinterpret_cast<uint4*>(ws + ChunkData<DELTA>::t01 + at * kStep + lane * 16) =
         make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
     *reinterpret_cast<uint2*>(ws + ChunkData<DELTA>::t2 + at * (kStep / 2) + lane * 8) =
@@ -455,12 +464,13 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
   __shared__ uint4 Uf[BUF][UP + 3][2][kWave];
   __shared__ uint4 Kt[KS][4][kWave];              // a state wave's dims of k, to be transposed
 
-  // the column tiles of a head on one XCD, whose L2 holds the head's chunk
+  // the column tiles of a head on one XCD, whose L2 then holds the head's
+  // chunk, and with enough of them the heads that share q and k
   const int tiles = a.dv / 16;
-  const int64_t heads = (int64_t)a.requests * a.v_heads;
   const int64_t in_xcd = blockIdx.x >> 3;
-  const int64_t head = in_xcd / tiles * 8 + (blockIdx.x & 7);
-  if (head >= heads) return;
+  const int64_t at_xcd = in_xcd / tiles;
+  const int64_t head = (at_xcd / a.span * 8 + (blockIdx.x & 7)) * a.span + at_xcd % a.span;
+  if (head >= (int64_t)a.requests * a.v_heads) return;
   const int tile = (int)(in_xcd % tiles);
   const int r = (int)(head / a.v_heads), hv = (int)(head - (int64_t)r * a.v_heads);
   const int hk = hv / (a.v_heads / a.k_heads);
@@ -569,6 +579,7 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
         for (int t = 0; t < 4; ++t) Kp[w4][t][lane] = x[t];
         lds_barrier();
       }
+      if constexpr (DELTA) lds_barrier();
       bf16x8 kt[2][2];
       transpose(now, kt);
       {
@@ -583,7 +594,6 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
       const float eC = now.eC;
       load(c + 2, now);
       lds_barrier();
-      if constexpr (DELTA) lds_barrier();
       uint4 uf[3][2];
 #pragma unroll
       for (int p = 2; p >= 0; --p)
@@ -683,8 +693,8 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
     for (int c = 0; c < chunks; ++c) {
       if constexpr (DELTA) {
         lds_barrier();
-        if (c > 0) finish(c - 1);
         lds_barrier();
+        if (c > 0) finish(c - 1);
         lds_barrier();
         take(0);
       } else {
@@ -805,6 +815,11 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
   if (c < chunks) step(c, even);
 }
 
+int64_t chunk_grid(const LinearArgs& a) {
+  const int64_t units = (int64_t)a.requests * a.v_heads / a.span;
+  return (units + 7) / 8 * 8 * a.span * (a.dv / 16);
+}
+
 template <int DK, bool DELTA>
 hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
   const int clear = a.clear ? kClearParts : 0;
@@ -818,9 +833,7 @@ hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
       <<<(unsigned)(a.chunks * a.v_heads + clear), kLinThreads, 0, s>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t heads = (int64_t)a.requests * a.v_heads;
-  linear_chunk_kernel<DK, DELTA>
-      <<<(unsigned)((heads + 7) / 8 * 8 * tiles), kChunkThreads, 0, s>>>(a);
+  linear_chunk_kernel<DK, DELTA><<<(unsigned)chunk_grid(a), kChunkThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -839,7 +852,10 @@ LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_head
   return l;
 }
 
-hipError_t launch_linear(const LinearArgs& a, hipStream_t s) {
+hipError_t launch_linear(const LinearArgs& in, hipStream_t s) {
+  LinearArgs a = in;
+  // fewer than eight key heads would leave XCDs idle
+  a.span = (int64_t)a.requests * a.k_heads >= 8 ? a.v_heads / a.k_heads : 1;
   if (a.dk == 64) return a.delta ? launch_linear_of<64, true>(a, s) : launch_linear_of<64, false>(a, s);
   return a.delta ? launch_linear_of<128, true>(a, s) : launch_linear_of<128, false>(a, s);
 }

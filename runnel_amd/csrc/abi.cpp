@@ -1190,8 +1190,8 @@ size_t rmoe_paged_attention_workspace_bytes(const rmoe_paged_cache* cache, int32
       q_heads % cache->kv_heads || requests < 1 || table_width < 0)
     return 0;
   const int splits =
-      rmoe::attention_splits(requests, cache->kv_heads, q_heads / cache->kv_heads,
-                             attention_keys(cache->page_size, table_width, window));
+      rmoe::attention_plan(requests, cache->kv_heads, q_heads / cache->kv_heads, cache->dim,
+                           attention_keys(cache->page_size, table_width, window)).splits;
   return attention_part_bytes((int64_t)requests * q_heads, splits, cache->dim, nullptr);
 }
 
@@ -1228,11 +1228,13 @@ int rmoe_paged_attention(const rmoe_rows* q, const rmoe_paged_cache* cache,
   a.lengths = lengths, a.window = window;
   a.scale_log2 = scale * (a.bits == 8 ? cache->k_scale : 1.0f) * 1.44269504088896f;
   a.v_scale = a.bits == 8 ? cache->v_scale : 1.0f;
-  a.splits = rmoe::attention_splits(requests, a.kv_heads, a.group,
-                                    attention_keys(cache->page_size, table_width, window));
+  const rmoe::AttentionPlan plan =
+      rmoe::attention_plan(requests, a.kv_heads, a.group, a.dim,
+                           attention_keys(cache->page_size, table_width, window));
+  a.splits = plan.splits, a.alone = plan.alone;
   a.out = out, a.lse = lse;
   const int64_t heads = (int64_t)requests * q->heads;
-  if (heads > kMaxGroups ||
+  if (heads * (a.dim / 32) > kMaxGroups ||
       (int64_t)requests * a.kv_heads * a.head_tiles * a.splits > kMaxGroups)
     return fail(RMOE_EINVAL, "too many requests times heads for one call");
   size_t ml;

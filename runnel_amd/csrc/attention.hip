@@ -38,8 +38,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kAttThreads = 256;
-constexpr int kAttWaves = kAttThreads / kWave;
+constexpr int kAttWaves = 4;  // of a workgroup that shares a request's keys with others
 constexpr int kAttTile = 32;  // keys of a step
 constexpr float kLn2 = 0.69314718056f;
 
@@ -143,9 +142,9 @@ __device__ __forceinline__ Share share_of(const AttentionArgs& a, int r) {
   return s;
 }
 
-template <int D, bool E4M3>
-__global__ __launch_bounds__(kAttThreads, D > 128 && !E4M3 ? 1 : 2) void attention_kernel(
-    const AttentionArgs a) {
+template <int D, bool E4M3, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, WAVES > 4 ? WAVES / 4 : D > 128 && !E4M3 ? 1 : 2)
+void attention_kernel(const AttentionArgs a) {
   constexpr int EB = E4M3 ? 1 : 2;    // bytes of a cached value
   constexpr int KS = D / 32;          // steps of the first product
   constexpr int NT = D / 16;          // tiles of the second
@@ -251,8 +250,8 @@ __global__ __launch_bounds__(kAttThreads, D > 128 && !E4M3 ? 1 : 2) void attenti
     load_k(t, pk);
     load_v(t, pv);
   }
-  for (; t < t_end; t += kAttWaves) {
-    const int next = t + kAttWaves;
+  for (; t < t_end; t += WAVES) {
+    const int next = t + WAVES;
     const int now_v[2] = {pv[0], pv[1]};
     if (next < t_end) pages(next, pk, pv);
 
@@ -362,67 +361,83 @@ __global__ __launch_bounds__(kAttThreads, D > 128 && !E4M3 ? 1 : 2) void attenti
     if (next < t_end) load_v(next, pv);
   }
 
-  // the four waves' parts together, a run of dims at a time
+  // the waves' parts together, a run of dims and four waves at a time
   l = head_sum(l);
-  float* ml = lds + kAttWaves * heads * P0;  // [wave][head] maximum, then sum
+  constexpr int THREADS = WAVES * kWave;
+  constexpr int ITEMS = (16 * P0 + THREADS - 1) / THREADS;  // of a thread: (head, dim) pairs
+  float* ml = lds + 4 * heads * P0;  // [wave][head] maximum, then sum
   if (n < heads && g == 0) {
     ml[wave * 16 + n] = m;
-    ml[(kAttWaves + wave) * 16 + n] = l;
+    ml[(WAVES + wave) * 16 + n] = l;
   }
   const int64_t row = (int64_t)r * a.kv_heads * a.group + head0;
   auto join = [&](auto run) {
     constexpr int P = decltype(run)::value ? P1 : P0, E = P / 16;
     constexpr int I0 = decltype(run)::value ? E0 : 0, D0 = decltype(run)::value ? P0 : 0;
-    if (n < heads) {
-      float* mine = lds + (wave * heads + n) * P + 4 * g * E;
+    float acc[ITEMS], sum[ITEMS], top[ITEMS];
 #pragma unroll
-      for (int i = 0; i < E; ++i)
+    for (int w0 = 0; w0 < WAVES; w0 += 4) {
+      if (w0 || D0) __syncthreads();
+      if (n < heads && wave >= w0 && wave < w0 + 4) {
+        float* mine = lds + ((wave - w0) * heads + n) * P + 4 * g * E;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mine[k * E + i] = o[I0 + i][k];
-    }
-    __syncthreads();
-    for (int i = tid; i < heads * P; i += kAttThreads) {
-      const int h = i / P, d = i - h * P;
-      float top = -INFINITY;
+        for (int i = 0; i < E; ++i)
 #pragma unroll
-      for (int w = 0; w < kAttWaves; ++w) top = fmaxf(top, ml[w * 16 + h]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, acc = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kAttWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ml[w * 16 + h] - base);
-        sum += f * ml[(kAttWaves + w) * 16 + h];
-        acc += f * lds[(w * heads + h) * P + d];
+          for (int k = 0; k < 4; ++k) mine[k * E + i] = o[I0 + i][k];
       }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < ITEMS; ++q) {
+        const int i = tid + q * THREADS;
+        if (i >= heads * P) continue;
+        const int h = i / P, d = i - h * P;
+        if (w0 == 0) {
+          acc[q] = sum[q] = 0.0f, top[q] = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < WAVES; ++w) top[q] = fmaxf(top[q], ml[w * 16 + h]);
+        }
+        const float base = top[q] == -INFINITY ? 0.0f : top[q];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = __builtin_amdgcn_exp2f(ml[(w0 + w) * 16 + h] - base);
+          sum[q] += f * ml[(WAVES + w0 + w) * 16 + h];
+          acc[q] += f * lds[(w * heads + h) * P + d];
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      const int i = tid + q * THREADS;
+      if (i >= heads * P) continue;
+      const int h = i / P, d = D0 + i - h * P;
       if (a.splits == 1) {
-        const bool some = sum > 0.0f || sum != sum;
-        a.out[(row + h) * D + D0 + d] =
-            (uint16_t)f32_to_bf16(some ? acc / sum * a.v_scale : 0.0f);
-        if (a.lse && D0 + d == 0)
-          a.lse[row + h] = top == -INFINITY ? top : (top + log2f(sum)) * kLn2;
+        const bool some = sum[q] > 0.0f || sum[q] != sum[q];
+        a.out[(row + h) * D + d] = (uint16_t)f32_to_bf16(some ? acc[q] / sum[q] * a.v_scale : 0.0f);
+        if (a.lse && d == 0)
+          a.lse[row + h] = top[q] == -INFINITY ? top[q] : (top[q] + log2f(sum[q])) * kLn2;
       } else {
         const int64_t part = (row + h) * a.splits + split;
-        a.part_o[part * D + D0 + d] = acc;
-        if (D0 + d == 0) a.part_ml[part] = make_float2(top, sum);
+        a.part_o[part * D + d] = acc[q];
+        if (d == 0) a.part_ml[part] = make_float2(top[q], sum[q]);
       }
     }
   };
   join(std::integral_constant<int, 0>());
-  if constexpr (P1 > 0) {
-    __syncthreads();
-    join(std::integral_constant<int, 1>());
-  }
+  if constexpr (P1 > 0) join(std::integral_constant<int, 1>());
 }
 
-// Joins the parts of one head: 256 threads, D / 4 of them across the dims
-// and the rest across the parts.
-template <int D>
+// Joins the parts of one head, or of 32 dims of it: SLICE / 4 threads across
+// the dims, the others across the parts.  Slices are for few heads, whose
+// parts are many (16 heads of 256 dims, 128 parts: 4.9 us, whole heads 6.7);
+// for many they are only more workgroups (1952 heads of 128 dims, 8 parts:
+// 13.2 us, whole heads 5.5).
+template <int D, int SLICE>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs a) {
-  constexpr int C = D / 4;          // threads across the dims
-  constexpr int Q = 256 / C;        // parts at a time
+  constexpr int C = SLICE / 4, Q = 256 / C, SLICES = D / SLICE;
   __shared__ float4 acc_s[Q][C];
   __shared__ float sum_s[Q];
-  const int64_t row = blockIdx.x;  // request and head
+  const int64_t row = blockIdx.x / SLICES;  // request and head
+  const int slice = blockIdx.x % SLICES;
   const int heads = a.kv_heads * a.group;
   const Share sh = share_of(a, (int)(row / heads));
   const int tid = threadIdx.x, c = tid % C, q = tid / C;
@@ -434,15 +449,16 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const float base = top == -INFINITY ? 0.0f : top;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-  if (q < Q) {
 #pragma unroll 4
-    for (int i = q; i < sh.parts; i += Q) {
-      const float2 e = ml[i];
-      const float f = __builtin_amdgcn_exp2f(e.x - base);
-      const float4 v = reinterpret_cast<const float4*>(a.part_o + (row * a.splits + i) * D)[c];
-      sum += f * e.y;
-      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-    }
+  for (int i = q; i < (q < Q ? sh.parts : 0); i += Q) {
+    const float2 e = ml[i];
+    const float f = __builtin_amdgcn_exp2f(e.x - base);
+    const float4 v =
+        reinterpret_cast<const float4*>(a.part_o + (row * a.splits + i) * D + slice * SLICE)[c];
+    sum += f * e.y;
+    acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+  }
+  if (q < Q) {
     acc_s[q][c] = acc;
     if (c == 0) sum_s[q] = sum;
   }
@@ -461,19 +477,33 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   uint2 w;
   w.x = f32_to_bf16(some ? acc.x * f : 0.0f) | f32_to_bf16(some ? acc.y * f : 0.0f) << 16;
   w.y = f32_to_bf16(some ? acc.z * f : 0.0f) | f32_to_bf16(some ? acc.w * f : 0.0f) << 16;
-  reinterpret_cast<uint2*>(a.out + row * D)[c] = w;
-  if (a.lse && tid == 0) a.lse[row] = top == -INFINITY ? top : (top + log2f(sum)) * kLn2;
+  reinterpret_cast<uint2*>(a.out + row * D + slice * SLICE)[c] = w;
+  if (a.lse && tid == 0 && slice == 0)
+    a.lse[row] = top == -INFINITY ? top : (top + log2f(sum)) * kLn2;
 }
+
+constexpr int kAloneWaves = 8;  // of a workgroup that has a request to itself
 
 template <int D, bool E4M3>
 hipError_t launch_attention_of(const AttentionArgs& a, hipStream_t s) {
   const int heads = a.group < 16 ? a.group : 16;
-  const size_t lds = (size_t)(kAttWaves * heads * Runs<D>::first + 2 * kAttWaves * 16) * sizeof(float);
-  const int64_t grid = (int64_t)a.requests * a.kv_heads * a.head_tiles * a.splits;
-  attention_kernel<D, E4M3><<<(unsigned)grid, kAttThreads, lds, s>>>(a);
-  hipError_t e = hipGetLastError();
+  const unsigned grid = (unsigned)((int64_t)a.requests * a.kv_heads * a.head_tiles * a.splits);
+  auto lds = [&](int waves) {
+    return (size_t)(4 * heads * Runs<D>::first + 2 * waves * 16) * sizeof(float);
+  };
+  if (a.alone) {
+    attention_kernel<D, E4M3, kAloneWaves>
+        <<<grid, kAloneWaves * kWave, lds(kAloneWaves), s>>>(a);
+    return hipGetLastError();
+  }
+  attention_kernel<D, E4M3, kAttWaves><<<grid, kAttWaves * kWave, lds(kAttWaves), s>>>(a);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  attention_join_kernel<D><<<(unsigned)(a.requests * a.kv_heads * a.group), 256, 0, s>>>(a);
+  const unsigned rows = (unsigned)(a.requests * a.kv_heads * a.group);
+  if (rows <= 256)
+    attention_join_kernel<D, 32><<<rows * (D / 32), 256, 0, s>>>(a);
+  else
+    attention_join_kernel<D, D><<<rows, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -484,15 +514,30 @@ hipError_t launch_attention_dim(const AttentionArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int attention_splits(int requests, int kv_heads, int group, int64_t keys) {
-  // two workgroups a compute unit where there are keys for them (a
-  // workgroup's four waves take a tile each at least)
+// Up to this many values of K a request that would be split is left whole to
+// one workgroup of eight waves, without a second launch (one request, 2 key
+// heads of 128 dims: 130 keys 8.6 us against 9.7, 500 keys 10.9 against 10.6,
+// and 4 us less on the host; 1000 keys 15.5 against 10.7: one compute unit
+// reads 60 GB/s).
+constexpr int64_t kAloneValues = 512 * 128;
+
+AttentionPlan attention_plan(int requests, int kv_heads, int group, int dim, int64_t keys) {
   const int64_t base = (int64_t)requests * kv_heads * ((group + 15) / 16);
   const int64_t tiles = (keys + kAttTile - 1) / kAttTile;
-  int64_t want = (512 + base - 1) / base;
+  if (base < 256 && tiles > kAttWaves && keys * dim <= kAloneValues) return {1, 1};
+  // a workgroup for every compute unit (131071 keys of 2 heads: 53 us at 128
+  // splits, 62 at 256); more where a request may be long, since the others
+  // may be short (61 requests of 17 to 16000 keys, 8 heads: 119 us at 2
+  // splits, 70 at 8); but no great many that find nothing to do (256 heads'
+  // worth of requests at 64 splits: half of the time)
+  int64_t want = (256 + base - 1) / base;
+  int64_t more = (keys + 2047) / 2048;
+  const int64_t most_groups = (8192 + base - 1) / base;
+  if (more > most_groups) more = most_groups;
+  if (more > want) want = more;
   const int64_t most = (tiles + kAttWaves - 1) / kAttWaves;
   want = want < most ? want : most;
-  return (int)(want < 1 ? 1 : want);
+  return {(int)(want < 1 ? 1 : want), 0};
 }
 
 hipError_t launch_attention(const AttentionArgs& in, hipStream_t s) {

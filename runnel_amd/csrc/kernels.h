@@ -266,12 +266,16 @@ struct AttentionArgs {
   int window;                 // 0: all keys
   float scale_log2, v_scale;  // k's scale and log2(e) are in the first
   int splits, least;          // workgroups of a request, tiles of each at least
+  int alone;                  // one workgroup of many waves instead
   uint16_t* out;              // [requests, kv_heads * group, dim]
   float* lse;                 // [requests, heads] or NULL
   float* part_o;              // [requests, heads, splits, dim] (splits > 1)
   float2* part_ml;            // [requests, heads, splits]
 };
-int attention_splits(int requests, int kv_heads, int group, int64_t keys);
+struct AttentionPlan {
+  int splits, alone;
+};
+AttentionPlan attention_plan(int requests, int kv_heads, int group, int dim, int64_t keys);
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t s);
 
 struct LinearArgs {

@@ -700,36 +700,50 @@ def dequantize(weight, scales, biases, bits: int, group_size: int = 64,
 E4M3 = torch.float8_e4m3fn
 
 
-def _one_device(*tensors) -> torch.device:
-    """The GPU all of the tensors are on; refuses tensors that want a gradient
-    (the operators below have no backward pass)."""
-    device = None
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
+_four = ctypes.c_int32 * 4
+
+
+def _one_device(*tensors) -> int:
+    """The index of the GPU that all of the tensors are on; refuses tensors
+    that want a gradient (the operators below have no backward pass)."""
+    index = None
     grad = torch.is_grad_enabled()
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError("runnel_amd kernels take GPU tensors")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"tensors are on {device} and {t.device}")
+        i = t.get_device()
+        if index is None:
+            index = i
+        elif i != index:
+            raise ValueError(f"tensors are on cuda:{index} and cuda:{i}")
         if grad and t.requires_grad:
             raise ValueError("this operator has no backward pass: call it under torch.no_grad() "
                              "or on detached tensors")
-    return device
+    return index
 
 
-def _there(device: torch.device):
-    """Makes `device` the current one for a launch."""
-    return torch.cuda.device(device.index)
+def _call(index: int, function, *args) -> None:
+    """`function` of the library, on GPU `index` and torch's current stream there."""
+    if index == _current_device():
+        rc = function(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = function(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _int32(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+    if t.dtype is torch.int32 and t.is_contiguous():
+        return t
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise ValueError(f"{name} must be int32 (got {t.dtype})")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
     return t.to(torch.int32).contiguous()
 
 
@@ -737,42 +751,47 @@ def _heads(t: torch.Tensor, name: str, rows: int | None = None, heads: int | Non
            dim: int | None = None):
     """A bf16 [rows, heads, dim] tensor and its rmoe_rows: as it lies where the
     kernels can read it so (a slice of a packed projection), else copied."""
-    if t.dtype != BF16 or t.dim() != 3:
+    shape = t.shape
+    if t.dtype is not BF16 or len(shape) != 3:
         raise ValueError(f"{name} must be a bfloat16 [rows, heads, dim] tensor "
-                         f"(got {t.dtype} {list(t.shape)})")
-    want = (t.shape[0] if rows is None else rows, t.shape[1] if heads is None else heads,
-            t.shape[2] if dim is None else dim)
-    if tuple(t.shape) != want:
-        raise ValueError(f"{name} must be {list(want)} (got {list(t.shape)})")
-    if (t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+                         f"(got {t.dtype} {list(shape)})")
+    if (rows is not None and shape[0] != rows or heads is not None and shape[1] != heads
+            or dim is not None and shape[2] != dim):
+        want = [n if m is None else m for n, m in zip(shape, (rows, heads, dim))]
+        raise ValueError(f"{name} must be {want} (got {list(shape)})")
+    row, head, one = t.stride()
+    address = t.data_ptr()
+    if one != 1 or row % 8 or head % 8 or address % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        if t.stride(0) % 8 or t.stride(1) % 8:
-            raise ValueError(f"{name}'s dim must be a multiple of 8 (got {t.shape[2]})")
-    return t, _lib.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1])
+        row, head, one = t.stride()
+        address = t.data_ptr()
+        if row % 8 or head % 8:
+            raise ValueError(f"{name}'s dim must be a multiple of 8 (got {shape[2]})")
+    return t, _lib.Rows(address, row, head, shape[1])
 
 
 def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: float,
            v_scale: float) -> _lib.PagedCache:
-    if k_cache.dtype not in (BF16, E4M3):
+    eight = k_cache.dtype is E4M3
+    if not eight and k_cache.dtype is not BF16:
         raise ValueError(f"the cache must be bfloat16 or float8_e4m3fn (got {k_cache.dtype})")
-    if k_cache.dim() != 4:
+    shape = k_cache.shape
+    if len(shape) != 4:
         raise ValueError("the cache must be [pages, kv heads, page size, dim] "
-                         f"(got {list(k_cache.shape)})")
-    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape:
+                         f"(got {list(shape)})")
+    if v_cache.dtype is not k_cache.dtype or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must have one type and shape")
-    pages, heads, size, dim = k_cache.shape
     # (a dimension of one has no stride)
-    ks, vs = ([0 if n == 1 else st for n, st in zip(c.shape, c.stride())]
-              for c in (k_cache, v_cache))
-    if ks != vs:
+    ks = [0 if n == 1 else st for n, st in zip(shape, k_cache.stride())]
+    if v_cache.stride() != k_cache.stride() and ks != [
+            0 if n == 1 else st for n, st in zip(shape, v_cache.stride())]:
         raise ValueError("k_cache and v_cache must lie in memory alike")
     if ks[3] != 1:
         raise ValueError("the cache's last dimension must be contiguous")
-    eight = k_cache.dtype == E4M3
     if not eight and (k_scale != 1.0 or v_scale != 1.0):
         raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], pages,
-                           size, heads, dim, 8 if eight else 16, k_scale, v_scale)
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], shape[0],
+                           shape[2], shape[1], shape[3], 8 if eight else 16, k_scale, v_scale)
 
 
 @dataclass
@@ -800,7 +819,8 @@ def paged_tables(cached: torch.Tensor, added: torch.Tensor, block_table: torch.T
     row count of the step's batch: tokens of all requests one after the
     other, rows behind the last one marked -1."""
     lib = _lib.load()
-    device = _one_device(cached, added, block_table, free_pages)
+    index = _one_device(cached, added, block_table, free_pages)
+    device = block_table.device
     if block_table.dtype != torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 [requests, pages]")
     R, P = block_table.shape
@@ -813,13 +833,11 @@ def paged_tables(cached: torch.Tensor, added: torch.Tensor, block_table: torch.T
     ints = torch.empty(2 * rows + 2 * R + 4, dtype=torch.int32, device=device)
     positions, requests, cu, lengths, counts = ints.split([rows, rows, R + 1, R, 3])
     slots = torch.empty(rows, dtype=torch.int64, device=device)
-    with _there(device):
-        _lib.check(lib.rmoe_paged_tables(
-            cached.data_ptr(), added.data_ptr(), R, block_table.data_ptr(),
-            max(block_table.stride(0), P) if R == 1 else block_table.stride(0), P,
-            free_pages.data_ptr(), free_pages.numel(), page_size, rows, slots.data_ptr(),
-            positions.data_ptr(), requests.data_ptr(), cu.data_ptr(), lengths.data_ptr(),
-            counts.data_ptr(), _lib.stream_handle(device)))
+    at = ints.data_ptr()
+    _call(index, lib.rmoe_paged_tables, cached.data_ptr(), added.data_ptr(), R,
+          block_table.data_ptr(), max(block_table.stride(0), P) if R == 1 else block_table.stride(0),
+          P, free_pages.data_ptr(), free_pages.numel(), page_size, rows, slots.data_ptr(), at,
+          at + 4 * rows, at + 8 * rows, at + 8 * rows + 4 * (R + 1), at + 8 * rows + 4 * (2 * R + 1))
     return PagedTables(slots, positions, requests, cu, lengths, counts)
 
 
@@ -828,15 +846,15 @@ def _rotary_spec(inv_freq, positions, rows: int, sections, woven: bool, adjacent
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float32 vector")
     half = inv_freq.numel()
-    sections = (half,) if sections is None else tuple(int(n) for n in sections)
-    if not 1 <= len(sections) <= 4:
-        raise ValueError(f"sections must name 1 to 4 axes (got {len(sections)})")
-    if positions.dim() == 1:
-        positions = positions[None]
-    positions = _int32(positions, "positions", (len(sections), rows))
-    spec = _lib.RotarySpec(inv_freq.data_ptr(), half, len(sections),
-                           (ctypes.c_int32 * 4)(*sections), int(bool(woven)),
-                           int(bool(adjacent)))
+    if sections is None:
+        sections = (half,)
+    axes = len(sections)
+    if not 1 <= axes <= 4:
+        raise ValueError(f"sections must name 1 to 4 axes (got {axes})")
+    positions = _int32(positions, "positions",
+                       (rows,) if axes == 1 and positions.dim() == 1 else (axes, rows))
+    spec = _lib.RotarySpec(inv_freq.data_ptr(), half, axes, _four(*sections), 1 if woven else 0,
+                           1 if adjacent else 0)
     return spec, positions
 
 
@@ -851,17 +869,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
     in turn when `woven` (axis i mod A until its section is used up, axis 0
     beyond)."""
     lib = _lib.load()
-    device = _one_device(q, k, positions, inv_freq)
+    index = _one_device(q, k, positions, inv_freq)
+    device = q.device
     q, qr = _heads(q, "q")
     k, kr = _heads(k, "k", q.shape[0], None, q.shape[2])
     spec, positions = _rotary_spec(inv_freq, positions, q.shape[0], sections, woven, adjacent)
     q_out = torch.empty(q.shape, dtype=BF16, device=device)
     k_out = torch.empty(k.shape, dtype=BF16, device=device)
-    with _there(device):
-        _lib.check(lib.rmoe_rotary(
-            ctypes.byref(spec), positions.data_ptr(), positions.stride(0), q.shape[0], q.shape[2],
-            ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), k_out.data_ptr(),
-            _lib.stream_handle(device)))
+    _call(index, lib.rmoe_rotary, ctypes.byref(spec), positions.data_ptr(), q.shape[0], q.shape[0],
+          q.shape[2], ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -876,25 +892,22 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     size + place, as ``paged_tables`` gives them; -1: nowhere) -> the turned q.
     8-bit caches hold e4m3(x / scale), saturating.  Slots of one call differ."""
     lib = _lib.load()
-    device = _one_device(q, k, v, positions, inv_freq, k_cache, v_cache, slots)
+    index = _one_device(q, k, v, positions, inv_freq, k_cache, v_cache, slots)
     cache = _cache(k_cache, v_cache, k_scale, v_scale)
-    for n, st in zip(k_cache.shape, k_cache.stride()):
-        if n > 1 and st == 0:
-            raise ValueError("an expanded cache cannot be written")
+    if 0 in k_cache.stride():
+        raise ValueError("an expanded cache cannot be written")
     q, qr = _heads(q, "q", None, None, cache.dim)
     N = q.shape[0]
     k, kr = _heads(k, "k", N, cache.kv_heads, cache.dim)
     v, vr = _heads(v, "v", N, cache.kv_heads, cache.dim)
     spec, positions = _rotary_spec(inv_freq, positions, N, sections, woven, adjacent)
-    if slots.dtype != torch.int64 or tuple(slots.shape) != (N,):
+    if slots.dtype is not torch.int64 or slots.shape != (N,):
         raise ValueError(f"slots must be int64 [{N}] (got {slots.dtype} {list(slots.shape)})")
     slots = slots.contiguous()
-    q_out = torch.empty(q.shape, dtype=BF16, device=device)
-    with _there(device):
-        _lib.check(lib.rmoe_rotary_append(
-            ctypes.byref(spec), positions.data_ptr(), positions.stride(0), N, ctypes.byref(qr),
-            q_out.data_ptr(), ctypes.byref(kr), ctypes.byref(vr), ctypes.byref(cache),
-            slots.data_ptr(), _lib.stream_handle(device)))
+    q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    _call(index, lib.rmoe_rotary_append, ctypes.byref(spec), positions.data_ptr(), N, N,
+          ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), ctypes.byref(vr),
+          ctypes.byref(cache), slots.data_ptr())
     return q_out
 
 
@@ -911,13 +924,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     count.  A request without keys gets zeros.  With return_lse also float32
     [R, Hq], the logarithm of the sum of the exponentials (-inf: no keys)."""
     lib = _lib.load()
-    device = _one_device(q, k_cache, v_cache, block_table, lengths)
+    index = _one_device(q, k_cache, v_cache, block_table, lengths)
+    device = q.device
     cache = _cache(k_cache, v_cache, k_scale, v_scale)
     q, qr = _heads(q, "q", None, None, cache.dim)
     R, heads, D = q.shape
     if block_table.dim() != 2 or block_table.shape[0] != R:
         raise ValueError(f"block_table must be [{R}, pages] (got {list(block_table.shape)})")
-    if block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+    if block_table.dtype is not torch.int32 or block_table.stride(1) != 1:
         block_table = _int32(block_table, "block_table", block_table.shape)
     lengths = _int32(lengths, "lengths", (R,))
     P = block_table.shape[1]
@@ -927,19 +941,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lse = torch.empty((R, heads), dtype=torch.float32, device=device) if return_lse else None
     need = lib.rmoe_paged_attention_workspace_bytes(ctypes.byref(cache), heads, R, P, window)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with _there(device):
-        _lib.check(lib.rmoe_paged_attention(
-            ctypes.byref(qr), ctypes.byref(cache), block_table.data_ptr(), block_table.stride(0),
-            P, lengths.data_ptr(), R, window, float(scale), out.data_ptr(), _lib.ptr(lse),
-            _lib.ptr(ws), need, _lib.stream_handle(device)))
+    _call(index, lib.rmoe_paged_attention, ctypes.byref(qr), ctypes.byref(cache),
+          block_table.data_ptr(), block_table.stride(0), P, lengths.data_ptr(), R, window, scale,
+          out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need)
     return (out, lse) if return_lse else out
 
 
 def _gate_rows(t: torch.Tensor, name: str, rows: int, heads: int) -> _lib.Gate:
-    if t.dtype != torch.float32 or tuple(t.shape) != (rows, heads):
+    if t.dtype is not torch.float32 or t.shape != (rows, heads):
         raise ValueError(f"{name} must be float32 [{rows}, {heads}] "
                          f"(got {t.dtype} {list(t.shape)})")
-    return _lib.Gate(t.data_ptr(), t.stride(0), t.stride(1))
+    return _lib.Gate(t.data_ptr(), *t.stride())
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -963,7 +975,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Calls of few tokens per sequence run token by token, others in chunks;
     both hold the state in float32."""
     lib = _lib.load()
-    device = _one_device(q, k, v, log_decay, cu_seqlens, state, beta, state_index, state_out)
+    index = _one_device(q, k, v, log_decay, cu_seqlens, state, beta, state_index, state_out)
+    device = q.device
     q, qr = _heads(q, "q")
     N, kh, dk = q.shape
     k, kr = _heads(k, "k", N, kh, dk)
@@ -975,20 +988,21 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     cu_seqlens = _int32(cu_seqlens, "cu_seqlens", (R + 1,))
     decay = _gate_rows(log_decay, "log_decay", N, vh)
     gate = None if beta is None else _gate_rows(beta, "beta", N, vh)
+    slots = state.shape[0] if state.dim() else 0
+    want = (slots, vh, dk, dv)
     if state_out is None:
         state_out = state
     for t, name in ((state, "state"), (state_out, "state_out")):
-        if (t.dtype != torch.float32 or t.dim() != 4 or tuple(t.shape[1:]) != (vh, dk, dv)
-                or t.shape[0] != state.shape[0] or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 [slots, {vh}, {dk}, {dv}] "
+        if t.dtype is not torch.float32 or t.shape != want or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 {list(want)} "
                              f"(got {t.dtype} {list(t.shape)})")
-    a, b, size = state.data_ptr(), state_out.data_ptr(), 4 * state.numel()
-    if a != b and a < b + size and b < a + size:
+    at, to = state.data_ptr(), state_out.data_ptr()
+    if at != to and abs(at - to) < 4 * state.numel():
         raise ValueError("state_out must be state or lie apart from it")
     if state_index is not None:
         state_index = _int32(state_index, "state_index", (R,))
-    elif state.shape[0] < R:
-        raise ValueError(f"state has {state.shape[0]} slots for {R} sequences")
+    elif slots < R:
+        raise ValueError(f"state has {slots} slots for {R} sequences")
     if scale is None:
         scale = dk ** -0.5
     if R == 0:
@@ -996,12 +1010,10 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     out = torch.empty((N, vh, dv), dtype=BF16, device=device)
     need = lib.rmoe_linear_attention_workspace_bytes(N, R, kh, vh, dk, int(gate is not None))
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with _there(device):
-        _lib.check(lib.rmoe_linear_attention(
-            ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr), ctypes.byref(decay),
-            None if gate is None else ctypes.byref(gate), cu_seqlens.data_ptr(), N, R, dk, dv,
-            float(scale), state.data_ptr(), state_out.data_ptr(), _lib.ptr(state_index),
-            state.shape[0], out.data_ptr(), 1, _lib.ptr(ws), need, _lib.stream_handle(device)))
+    _call(index, lib.rmoe_linear_attention, ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr),
+          ctypes.byref(decay), None if gate is None else ctypes.byref(gate), cu_seqlens.data_ptr(),
+          N, R, dk, dv, scale, at, to, _lib.ptr(state_index), slots, out.data_ptr(), 1,
+          _lib.ptr(ws), need)
     return out
 
 

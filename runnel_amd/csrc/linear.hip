@@ -73,17 +73,23 @@ __device__ void clear_uncovered(const LinearArgs& a, int part, int parts) {
   for (int64_t i = hi + at; i < end; i += step) o[i] = z;
 }
 
+// 32-column waves from which the token form takes them (2048: 13.2 us against
+// 12.8 with twice as many of 16, 4096: 28 against 31)
+constexpr int64_t kWideStates = 4096;
 constexpr int kClearParts = 16;  // workgroups that look for uncovered rows
 
 // ------------------------------------------------------------ token by token
-// A wave holds 16 columns of a state: lane (rg, c) the rows rg DK/16 .. of
+// A wave holds 4 LC columns of a state: lane (rg, c) the rows rg RW .. of
 // columns 4 c .. 4 c + 3.  Both sums over the rows, S^T k and S^T q, are of
 // the state before the token, so a token costs one round of exchanges:
-// o = a S^T q + (q.k) u.
-template <int DK, bool DELTA>
+// o = a S^T q + (q.k) u.  Bound by the state's read and write; LC 8 moves
+// whole lines (127 tokens x 32 heads of 128 x 128: 106 us, 5.0 TB/s, against
+// 121 with LC 4 and 108 with 16), LC 4 has twice the waves for few states (one
+// token x 32 heads: 5.0 us against 5.6).
+template <int DK, bool DELTA, int LC>
 __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearArgs a) {
-  constexpr int RW = DK / 16;  // rows of a lane
-  const int tiles = a.dv / 16;
+  constexpr int RW = DK * LC / kWave;  // rows of a lane
+  const int tiles = a.dv / (4 * LC);
   const int64_t waves = (int64_t)a.requests * a.v_heads * tiles;
   const int64_t groups = (waves + 3) / 4;
   if (blockIdx.x >= groups) {
@@ -92,12 +98,12 @@ __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearAr
   }
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (id >= waves) return;
-  const int lane = threadIdx.x & 63, c = lane & 3, rg = lane >> 2;
+  const int lane = threadIdx.x & 63, c = lane % LC, rg = lane / LC;
   const int tile = (int)(id % tiles);
   const int hv = (int)(id / tiles % a.v_heads);
   const int r = (int)(id / tiles / a.v_heads);
   const int hk = hv / (a.v_heads / a.k_heads);
-  const int col = tile * 16 + c * 4;
+  const int col = (tile * LC + c) * 4;
   const int64_t slot = slot_of(a, r);
   const int64_t at = ((slot * a.v_heads + hv) * DK + rg * RW) * a.dv + col;
   f32x4 s[RW];
@@ -140,7 +146,7 @@ __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearAr
       qk = fmaf(qv[i], kv[i], qk);
     }
 #pragma unroll
-    for (int d = 4; d < kWave; d <<= 1) {
+    for (int d = LC; d < kWave; d <<= 1) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (DELTA) sk[j] += __shfl_xor(sk[j], d, kWave);
@@ -823,10 +829,16 @@ int64_t chunk_grid(const LinearArgs& a) {
 template <int DK, bool DELTA>
 hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
   const int clear = a.clear ? kClearParts : 0;
-  const int64_t tiles = a.dv / 16;
   if (!a.workspace) {
-    const int64_t waves = (int64_t)a.requests * a.v_heads * tiles;
-    linear_step_kernel<DK, DELTA><<<(unsigned)((waves + 3) / 4 + clear), kLinThreads, 0, s>>>(a);
+    const int64_t wide = (int64_t)a.requests * a.v_heads * (a.dv / 32);
+    if (a.dv % 32 == 0 && wide >= kWideStates) {
+      linear_step_kernel<DK, DELTA, 8>
+          <<<(unsigned)((wide + 3) / 4 + clear), kLinThreads, 0, s>>>(a);
+    } else {
+      const int64_t waves = (int64_t)a.requests * a.v_heads * (a.dv / 16);
+      linear_step_kernel<DK, DELTA, 4>
+          <<<(unsigned)((waves + 3) / 4 + clear), kLinThreads, 0, s>>>(a);
+    }
     return hipGetLastError();
   }
   linear_prepare_kernel<DK, DELTA>

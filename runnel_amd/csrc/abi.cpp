@@ -1308,7 +1308,7 @@ int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_row
       rmoe::linear_layout(tokens, requests, a.k_heads, a.v_heads, dk, a.delta);
   // workgroups of 768 threads, for whole eights of key heads
   const int64_t tiles = ((int64_t)requests * a.k_heads + 8) * (a.v_heads / a.k_heads) * (dv / 16);
-  if (tiles > kMaxGroups / 3 || l.chunks * a.v_heads + 64 > kMaxGroups)
+  if (tiles > kMaxGroups / 3 || l.chunks * a.v_heads + tiles + 64 > kMaxGroups)
     return fail(RMOE_EINVAL, "too many sequences, tokens or heads for one call");
   if (rmoe::linear_in_chunks(tokens, requests)) {
     if (!workspace || workspace_bytes < (size_t)l.total)
@@ -1316,6 +1316,8 @@ int rmoe_linear_attention(const rmoe_rows* q, const rmoe_rows* k, const rmoe_row
                   workspace_bytes);
     if (!aligned(workspace, 16)) return fail(RMOE_EALIGN, "workspace must be 16-byte aligned");
     a.workspace = workspace, a.chunks = l.chunks, a.key_offset = l.key_offset;
+    if (requests > 1)
+      a.list = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + l.list_offset);
   }
   const hipError_t e = rmoe::launch_linear(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "linear attention launch");

@@ -295,10 +295,12 @@ struct LinearArgs {
   int clear;                  // rows of no sequence are set to zero
   void* workspace;            // NULL: token by token
   int64_t chunks, key_offset;
+  int32_t* list;              // sequences that go in chunks (NULL: the only one, or none)
+  int by_token;               // tokens up to which one does not (set by launch_linear)
   int span;                   // value heads side by side on an XCD (set by launch_linear)
 };
 struct LinearLayout {
-  int64_t chunks, key_offset, total;
+  int64_t chunks, key_offset, list_offset, total;
 };
 bool linear_in_chunks(int64_t tokens, int requests);
 LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_heads, int dk,

@@ -78,7 +78,55 @@ __device__ void clear_uncovered(const LinearArgs& a, int part, int parts) {
 constexpr int64_t kWideStates = 4096;
 constexpr int kClearParts = 16;  // workgroups that look for uncovered rows
 
+// The sequences that go in chunks, more than a.by_token tokens: list[0] is their
+// count, their numbers are from list[1] on, those with more chunks (by
+// powers of two) first, so that the longest do not start last.  One workgroup.
+__device__ void list_long(const LinearArgs& a) {
+  __shared__ int counts[2][kLinThreads / kWave];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto length = [&](int r) { return r < a.requests ? seq_of(a, r).len : 0; };
+  const bool few = a.requests <= kLinThreads;  // each thread's length stays with it
+  const int first = few ? length(tid) : 0;
+  int at = 0, turn = 0;
+  for (int level = 31 - __clz((a.tokens + 63) / 64); level >= 0; --level) {
+    for (int r0 = 0; r0 < a.requests; r0 += kLinThreads, turn ^= 1) {
+      const int r = r0 + tid;
+      const int len = few ? first : length(r);
+      const bool mine = len > a.by_token && 31 - __clz((len + 63) / 64) == level;
+      const uint64_t mask = __ballot(mine);
+      if (lane == 0) counts[turn][wave] = __popcll(mask);
+      __syncthreads();
+      int before = 0, all = 0;
+      for (int w = 0; w < kLinThreads / kWave; ++w) {
+        before += w < wave ? counts[turn][w] : 0;
+        all += counts[turn][w];
+      }
+      if (mine) a.list[1 + at + before + __popcll(mask & ((1ull << lane) - 1))] = r;
+      at += all;
+    }
+  }
+  if (tid == 0) a.list[0] = at;
+}
+
 // ------------------------------------------------------------ token by token
+// Sum over the lanes equal modulo LC (4, 8 or 16): rotations inside 16 lanes,
+// then the swaps across them, all without LDS.
+template <int LC>
+__device__ __forceinline__ float sum_over_rows(float v) {
+  if constexpr (LC < 16)  // row_ror:8
+    v += __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, false));
+  if constexpr (LC < 8)  // row_ror:4
+    v += __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xF, 0xF, false));
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const uint32_t w = __float_as_uint(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // A wave holds 4 LC columns of a state: lane (rg, c) the rows rg RW .. of
 // columns 4 c .. 4 c + 3.  Both sums over the rows, S^T k and S^T q, are of
 // the state before the token, so a token costs one round of exchanges:
@@ -87,23 +135,19 @@ constexpr int kClearParts = 16;  // workgroups that look for uncovered rows
 // 121 with LC 4 and 108 with 16), LC 4 has twice the waves for few states (one
 // token x 32 heads: 5.0 us against 5.6).
 template <int DK, bool DELTA, int LC>
-__global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearArgs a) {
+__device__ __forceinline__ void by_token(const LinearArgs& a, int64_t group) {
   constexpr int RW = DK * LC / kWave;  // rows of a lane
   const int tiles = a.dv / (4 * LC);
-  const int64_t waves = (int64_t)a.requests * a.v_heads * tiles;
-  const int64_t groups = (waves + 3) / 4;
-  if (blockIdx.x >= groups) {
-    clear_uncovered(a, (int)(blockIdx.x - groups), kClearParts);
-    return;
-  }
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= waves) return;
+  const int64_t id = group * 4 + (threadIdx.x >> 6);
+  if (id >= (int64_t)a.requests * a.v_heads * tiles) return;
   const int lane = threadIdx.x & 63, c = lane % LC, rg = lane / LC;
   const int tile = (int)(id % tiles);
   const int hv = (int)(id / tiles % a.v_heads);
   const int r = (int)(id / tiles / a.v_heads);
   const int hk = hv / (a.v_heads / a.k_heads);
   const int col = (tile * LC + c) * 4;
+  const Seq q = seq_of(a, r);
+  if (a.list && q.len > a.by_token) return;
   const int64_t slot = slot_of(a, r);
   const int64_t at = ((slot * a.v_heads + hv) * DK + rg * RW) * a.dv + col;
   f32x4 s[RW];
@@ -111,29 +155,46 @@ __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearAr
   for (int i = 0; i < RW; ++i)
     s[i] = slot >= 0 ? *reinterpret_cast<const f32x4*>(a.state + at + (int64_t)i * a.dv)
                      : (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  const Seq q = seq_of(a, r);
-  for (int t = 0; t < q.len; ++t) {
-    const int64_t row = q.begin + t;
+  // a token's inputs, asked for while the one before is worked on
+  struct Token {
+    uint2 k[RW / 4], q[RW / 4];
+    uint16_t v[4];
+    float g, beta;
+  };
+  auto load = [&](int t) {
+    Token x;
+    const int64_t row = q.begin + (t < q.len ? t : q.len - 1);
     const uint16_t* kp = a.k + row * a.k_row + hk * a.k_head + rg * RW;
     const uint16_t* qp = a.q + row * a.q_row + hk * a.q_head + rg * RW;
-    float kv[RW], qv[RW];
-#pragma unroll
-    for (int i = 0; i < RW; i += 4) {
-      const uint2 ku = *reinterpret_cast<const uint2*>(kp + i);
-      const uint2 qu = *reinterpret_cast<const uint2*>(qp + i);
-      kv[i] = bf16_lo(ku.x), kv[i + 1] = bf16_hi(ku.x);
-      kv[i + 2] = bf16_lo(ku.y), kv[i + 3] = bf16_hi(ku.y);
-      qv[i] = bf16_lo(qu.x), qv[i + 1] = bf16_hi(qu.x);
-      qv[i + 2] = bf16_lo(qu.y), qv[i + 3] = bf16_hi(qu.y);
-    }
     const uint16_t* vp = a.v + row * a.v_row + hv * a.v_head + col;
-    float u[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = bf16_to_f32(vp[j]);
-    const float g = log_decay(a, row, hv);
-    const float decay = expf(g);
-    float beta = 1.0f;
-    if constexpr (DELTA) beta = a.beta[row * a.beta_row + hv * a.beta_head];
+    for (int i = 0; i < RW / 4; ++i) {
+      x.k[i] = reinterpret_cast<const uint2*>(kp)[i];
+      x.q[i] = reinterpret_cast<const uint2*>(qp)[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] = vp[j];
+    x.g = log_decay(a, row, hv);
+    x.beta = DELTA ? a.beta[row * a.beta_row + hv * a.beta_head] : 1.0f;
+    return x;
+  };
+  Token next;
+  if (q.len > 0) next = load(0);
+  for (int t = 0; t < q.len; ++t) {
+    const int64_t row = q.begin + t;
+    const Token x = next;
+    if (q.len > 1) next = load(t + 1);
+    float kv[RW], qv[RW], u[4];
+#pragma unroll
+    for (int i = 0; i < RW / 4; ++i) {
+      kv[4 * i] = bf16_lo(x.k[i].x), kv[4 * i + 1] = bf16_hi(x.k[i].x);
+      kv[4 * i + 2] = bf16_lo(x.k[i].y), kv[4 * i + 3] = bf16_hi(x.k[i].y);
+      qv[4 * i] = bf16_lo(x.q[i].x), qv[4 * i + 1] = bf16_hi(x.q[i].x);
+      qv[4 * i + 2] = bf16_lo(x.q[i].y), qv[4 * i + 3] = bf16_hi(x.q[i].y);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = bf16_to_f32(x.v[j]);
+    const float decay = expf(x.g), beta = x.beta;
 
     float sk[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sq[4] = {0.0f, 0.0f, 0.0f, 0.0f}, qk = 0.0f;
 #pragma unroll
@@ -146,14 +207,11 @@ __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearAr
       qk = fmaf(qv[i], kv[i], qk);
     }
 #pragma unroll
-    for (int d = LC; d < kWave; d <<= 1) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (DELTA) sk[j] += __shfl_xor(sk[j], d, kWave);
-        sq[j] += __shfl_xor(sq[j], d, kWave);
-      }
-      qk += __shfl_xor(qk, d, kWave);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DELTA) sk[j] = sum_over_rows<LC>(sk[j]);
+      sq[j] = sum_over_rows<LC>(sq[j]);
     }
+    qk = sum_over_rows<LC>(qk);
     if constexpr (DELTA) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) u[j] = beta * (u[j] - decay * sk[j]);
@@ -176,8 +234,23 @@ __global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearAr
     *reinterpret_cast<f32x4*>(a.state_out + at + (int64_t)i * a.dv) = s[i];
 }
 
+// Workgroups that take all sequences by token, 4 LC columns a wave.
+__host__ __device__ __forceinline__ int64_t token_groups(const LinearArgs& a, int lc) {
+  return ((int64_t)a.requests * a.v_heads * (a.dv / (4 * lc)) + 3) / 4;
+}
+
+template <int DK, bool DELTA, int LC>
+__global__ __launch_bounds__(kLinThreads) void linear_step_kernel(const LinearArgs a) {
+  const int64_t groups = token_groups(a, LC);
+  if (blockIdx.x < groups)
+    by_token<DK, DELTA, LC>(a, blockIdx.x);
+  else
+    clear_uncovered(a, (int)(blockIdx.x - groups), kClearParts);
+}
+
 // ------------------------------------------------------------------ in chunks
 constexpr int kChunk = 64;
+constexpr int kFewTokens = 8;
 constexpr int kChunkThreads = 12 * kWave;
 constexpr int kStep = 1024;  // bytes of one operand A of 16 x 32 values, in lane order
 
@@ -261,7 +334,7 @@ __device__ __forceinline__ void lds_barrier() {
 // wave loads its own 16 rows of k and takes the others' from LDS (from memory
 // each tile was a wait of its own); exponentials are of sums kept in base 2.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const LinearArgs a) {
+__device__ __forceinline__ void prepare(const LinearArgs& a, int64_t block) {
   constexpr int KS = DK / 32;
   constexpr int LD = 20;              // row of a 16 x 16 tile in LDS
   constexpr int TILE = 16 * LD;
@@ -272,13 +345,8 @@ __global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const Li
   constexpr int SHARED = KS * 4 * kWave * 4;
   __shared__ __align__(16) float Ts[SHARED > kTiles * TILE ? SHARED : kTiles * TILE];
 
-  const int64_t blocks = a.chunks * a.v_heads;
-  if (blockIdx.x >= blocks) {
-    clear_uncovered(a, (int)(blockIdx.x - blocks), kClearParts);
-    return;
-  }
-  const int64_t c = blockIdx.x / a.v_heads;
-  const int hv = (int)(blockIdx.x - c * a.v_heads);
+  const int64_t c = block / a.v_heads;
+  const int hv = (int)(block - c * a.v_heads);
   const int each = a.v_heads / a.k_heads;
   const int hk = hv / each;
   int r = 0, hi = a.requests;  // the last r whose chunks start at or before c
@@ -291,7 +359,7 @@ __global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const Li
   }
   const Seq sq = seq_of(a, r);
   const int64_t first = (c - chunk_base(a, r)) * kChunk;
-  if (first < 0 || first >= sq.len) return;
+  if (first < 0 || first >= sq.len || (a.list && sq.len <= a.by_token)) return;
   const int64_t row0 = sq.begin + first;
   const int len = (int)(sq.len - first < kChunk ? sq.len - first : kChunk);
 
@@ -443,6 +511,24 @@ __global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const Li
   }
 }
 
+// The first launch of a call in chunks: the preparation of every chunk, and
+// where lengths may differ the short sequences (whole, by token) and the list
+// of the others beside it.
+template <int DK, bool DELTA>
+__global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const LinearArgs a) {
+  int64_t block = blockIdx.x;
+  if (a.list) {
+    if (block == 0) return list_long(a);
+    block -= 1;
+    const int64_t groups = token_groups(a, 4);
+    if (block < groups) return by_token<DK, DELTA, 4>(a, block);
+    block -= groups;
+  }
+  const int64_t chunks = a.chunks * a.v_heads;
+  if (block < chunks) return prepare<DK, DELTA>(a, block);
+  clear_uncovered(a, (int)(block - chunks), kClearParts);
+}
+
 // One (sequence, head, 16 columns of the state) from chunk to chunk, twelve
 // waves, three to a SIMD (one alone waits between its instructions):
 //
@@ -459,7 +545,7 @@ __global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const Li
 // chain (outputs, q S, turning k, loads) is done by whoever is not in it.
 // Without it U is v, and one exchange is left.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const LinearArgs a) {
+__device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int hv, int tile) {
   constexpr int KS = DK / 32;         // state waves
   constexpr int SP = DELTA ? 3 : 2;   // pieces of the state that a product takes
   constexpr int UP = DELTA ? 2 : 1;   // of U in P U (v alone is bf16 as it is)
@@ -470,15 +556,6 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
   __shared__ uint4 Uf[BUF][UP + 3][2][kWave];
   __shared__ uint4 Kt[KS][4][kWave];              // a state wave's dims of k, to be transposed
 
-  // the column tiles of a head on one XCD, whose L2 then holds the head's
-  // chunk, and with enough of them the heads that share q and k
-  const int tiles = a.dv / 16;
-  const int64_t in_xcd = blockIdx.x >> 3;
-  const int64_t at_xcd = in_xcd / tiles;
-  const int64_t head = (at_xcd / a.span * 8 + (blockIdx.x & 7)) * a.span + at_xcd % a.span;
-  if (head >= (int64_t)a.requests * a.v_heads) return;
-  const int tile = (int)(in_xcd % tiles);
-  const int r = (int)(head / a.v_heads), hv = (int)(head - (int64_t)r * a.v_heads);
   const int hk = hv / (a.v_heads / a.k_heads);
   const Seq sq = seq_of(a, r);
   const int64_t slot = slot_of(a, r);
@@ -821,37 +898,81 @@ __global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const Linea
   if (c < chunks) step(c, even);
 }
 
-int64_t chunk_grid(const LinearArgs& a) {
-  const int64_t units = (int64_t)a.requests * a.v_heads / a.span;
+// The column tiles of a head on one XCD, whose L2 then holds the head's chunk,
+// and with enough of them the heads that share q and k.
+__host__ __device__ __forceinline__ int64_t chunk_items(const LinearArgs& a, int64_t sequences) {
+  const int64_t units = sequences * a.v_heads / a.span;
   return (units + 7) / 8 * 8 * a.span * (a.dv / 16);
 }
+
+template <int DK, bool DELTA>
+__device__ __forceinline__ void chunk_item(const LinearArgs& a, int64_t id, int count) {
+  const int tiles = a.dv / 16;
+  const int64_t in_xcd = id >> 3;
+  const int64_t at_xcd = in_xcd / tiles;
+  const int64_t head = (at_xcd / a.span * 8 + (id & 7)) * a.span + at_xcd % a.span;
+  if (head >= (int64_t)count * a.v_heads) return;
+  const int which = (int)(head / a.v_heads);
+  through_chunks<DK, DELTA>(a, a.list ? a.list[1 + which] : 0,
+                            (int)(head - (int64_t)which * a.v_heads), (int)(in_xcd % tiles));
+}
+
+// A workgroup takes one item of the only sequence, or of listed ones its item
+// and those a grid further on, which are on the same XCD.  (The loop costs the
+// chunks 8% of their time in registers: 8192 tokens x 32 heads 230 us for 213.)
+template <int DK, bool DELTA, bool LISTED>
+__global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const LinearArgs a) {
+  if constexpr (!LISTED) {
+    chunk_item<DK, DELTA>(a, blockIdx.x, 1);
+  } else {
+    const int count = a.list[0];
+    const int64_t items = chunk_items(a, count);
+    for (int64_t id = blockIdx.x; id < items; id += gridDim.x) {
+      chunk_item<DK, DELTA>(a, id, count);
+      lds_barrier();  // the next one's first exchange writes where this one's last is read
+    }
+  }
+}
+// Workgroups of the chunk kernel: one a compute unit is all that its registers
+// allow, and a workgroup without work would cost a turn.
+constexpr int64_t kChunkGroups = 256;
 
 template <int DK, bool DELTA>
 hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
   const int clear = a.clear ? kClearParts : 0;
   if (!a.workspace) {
-    const int64_t wide = (int64_t)a.requests * a.v_heads * (a.dv / 32);
-    if (a.dv % 32 == 0 && wide >= kWideStates) {
+    if (a.dv % 32 == 0 && (int64_t)a.requests * a.v_heads * (a.dv / 32) >= kWideStates)
       linear_step_kernel<DK, DELTA, 8>
-          <<<(unsigned)((wide + 3) / 4 + clear), kLinThreads, 0, s>>>(a);
-    } else {
-      const int64_t waves = (int64_t)a.requests * a.v_heads * (a.dv / 16);
+          <<<(unsigned)(token_groups(a, 8) + clear), kLinThreads, 0, s>>>(a);
+    else
       linear_step_kernel<DK, DELTA, 4>
-          <<<(unsigned)((waves + 3) / 4 + clear), kLinThreads, 0, s>>>(a);
-    }
+          <<<(unsigned)(token_groups(a, 4) + clear), kLinThreads, 0, s>>>(a);
     return hipGetLastError();
   }
+  const int64_t beside = a.list ? 1 + token_groups(a, 4) : 0;
   linear_prepare_kernel<DK, DELTA>
-      <<<(unsigned)(a.chunks * a.v_heads + clear), kLinThreads, 0, s>>>(a);
+      <<<(unsigned)(beside + a.chunks * a.v_heads + clear), kLinThreads, 0, s>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  linear_chunk_kernel<DK, DELTA><<<(unsigned)chunk_grid(a), kChunkThreads, 0, s>>>(a);
+  if (!a.list) {
+    linear_chunk_kernel<DK, DELTA, false>
+        <<<(unsigned)chunk_items(a, 1), kChunkThreads, 0, s>>>(a);
+    return hipGetLastError();
+  }
+  const int64_t most = a.tokens / (a.by_token + 1);  // sequences that go in chunks
+  const int64_t items = chunk_items(a, most < a.requests ? most : a.requests);
+  linear_chunk_kernel<DK, DELTA, true>
+      <<<(unsigned)(items < kChunkGroups ? items : kChunkGroups), kChunkThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-bool linear_in_chunks(int64_t tokens, int requests) { return tokens > 16 * (int64_t)requests; }
+// Of several sequences, none empty, the longest has at most tokens - requests
+// + 1 tokens.
+bool linear_in_chunks(int64_t tokens, int requests) {
+  return requests == 1 ? tokens > kFewTokens : tokens - requests > 32;
+}
 
 LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_heads, int dk,
                            bool delta) {
@@ -859,15 +980,22 @@ LinearLayout linear_layout(int64_t tokens, int requests, int k_heads, int v_head
   l.chunks = tokens / kChunk + requests;
   l.key_offset = l.chunks * v_heads *
                  (int64_t)(delta ? ChunkData<true>::bytes : ChunkData<false>::bytes);
-  l.total = l.key_offset + l.chunks * k_heads *
-                               (int64_t)(dk == 64 ? KeyData<64>::bytes : KeyData<128>::bytes);
+  l.list_offset = l.key_offset + l.chunks * k_heads *
+                                     (int64_t)(dk == 64 ? KeyData<64>::bytes : KeyData<128>::bytes);
+  l.total = l.list_offset + (requests > 1 ? ((int64_t)requests + 1) * 4 : 0);
   return l;
 }
 
 hipError_t launch_linear(const LinearArgs& in, hipStream_t s) {
   LinearArgs a = in;
+  // Where lengths may differ, which sequences are taken by token.  Few states
+  // leave most of the chip to a sequence's chunks, and a token costs its wave
+  // 0.9 us (one sequence x 32 heads of 128 x 128: 8 tokens 10.8 us and 12.5 in
+  // chunks, 16 tokens 18.8 and 12.6); many fill it either way (16 sequences:
+  // 24 tokens 58 and 68, 32 tokens 73 and 67; 64: 64 tokens 356 and 301).
+  a.by_token = (int64_t)a.requests * a.v_heads * (a.dv / 16) >= 4096 ? 24 : kFewTokens;
   // fewer than eight key heads would leave XCDs idle
-  a.span = (int64_t)a.requests * a.k_heads >= 8 ? a.v_heads / a.k_heads : 1;
+  a.span = a.k_heads >= 8 ? a.v_heads / a.k_heads : 1;
   if (a.dk == 64) return a.delta ? launch_linear_of<64, true>(a, s) : launch_linear_of<64, false>(a, s);
   return a.delta ? launch_linear_of<128, true>(a, s) : launch_linear_of<128, false>(a, s);
 }

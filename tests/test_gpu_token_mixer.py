@@ -448,6 +448,17 @@ def test_linear_chunks(native, lens, delta):
 
 
 @pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("R", [3, 300])
+def test_linear_mixed(native, R, delta):
+    """Single tokens, a few and prompts in one batch: by token and in chunks
+    in one call, with 300 sequences more than a workgroup lists at once."""
+    lens = [[1, 9, 70], [0, 8, 33], [130, 2, 1]][R % 3] if R == 3 else [
+        (1, 24, 0, 25, 1, 2, 65, 1, 1, 17)[i * 7 % 10] for i in range(R)]
+    kh, vh, dv = (1, 2, 16) if R == 3 else (2, 4, 64)
+    check_linear(native, *linear_inputs(R, lens, kh, vh, 64, dv, delta))
+
+
+@pytest.mark.parametrize("delta", [True, False])
 @pytest.mark.parametrize("decay", [0.0, -1e-4, -0.3, -40.0, -float("inf")])
 def test_linear_decays(native, decay, delta):
     """One rate for a head, expanded over the tokens: none, slow, and so

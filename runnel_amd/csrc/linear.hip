@@ -551,7 +551,10 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
   constexpr int UP = DELTA ? 2 : 1;   // of U in P U (v alone is bf16 as it is)
   constexpr int BUF = DELTA ? 1 : 2;  // one exchange a chunk: two buffers in turn
   __shared__ f32x4 Kp[DELTA ? KS : 1][4][kWave];  // partial K S of each 16 tokens
-  __shared__ f32x4 Qp[BUF][KS][4][kWave];         // and Q S
+  // q S: of the output waves, from two pieces of the state; without beta, where
+  // they are the busiest, of the state waves, in parts
+  __shared__ uint4 Sf[2][KS][kWave];
+  __shared__ f32x4 Qp[BUF][DELTA ? 1 : KS][4][kWave];
   __shared__ uint4 Rf[DELTA ? 3 : 1][2][kWave];
   __shared__ uint4 Uf[BUF][UP + 3][2][kWave];
   __shared__ uint4 Kt[KS][4][kWave];              // a state wave's dims of k, to be transposed
@@ -601,17 +604,19 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
                        (c0 * a.k_heads + hk) * (int64_t)KeyData<DK>::bytes + w4 * 4 * kStep;
     const int64_t key_step = (int64_t)a.k_heads * KeyData<DK>::bytes;
     struct Loads {
-      uint4 k[4], q[4];
+      uint4 k[4], q[DELTA ? 1 : 4];
       float eC;
     };
-    // the wave's dims of 64 tokens of k and of q
+    // the wave's dims of 64 tokens of k and, without beta, of q
     auto load = [&](int c, Loads& x) {
       c = clamped(c);
       const char* k = key0 + c * key_step;
 #pragma unroll
       for (int t = 0; t < 4; ++t) x.k[t] = load16(k + KeyData<DK>::k + t * kStep + l16);
+      if constexpr (!DELTA) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) x.q[t] = load16(k + KeyData<DK>::q + t * kStep + l16);
+        for (int t = 0; t < 4; ++t) x.q[t] = load16(k + KeyData<DK>::q + t * kStep + l16);
+      }
       x.eC = *reinterpret_cast<const float*>(ws0 + c * ws_step + ChunkData<DELTA>::state +
                                              128 * w4 + 4 * (uint32_t)(lane >> 6));
     };
@@ -661,11 +666,16 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
 #pragma unroll
         for (int t = 0; t < 4; ++t) Kp[w4][t][lane] = x[t];
         lds_barrier();
+        __builtin_amdgcn_s_setprio(0);  // out of the chain until U is there
       }
-      if constexpr (DELTA) lds_barrier();
       bf16x8 kt[2][2];
-      transpose(now, kt);
-      {
+      if constexpr (DELTA) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) *reinterpret_cast<bf16x8*>(&Sf[p][w4][lane]) = sf[p];
+        lds_barrier();
+        transpose(now, kt);
+      } else {
+        transpose(now, kt);
         f32x4 x[4] = {};
 #pragma unroll
         for (int p = 1; p >= 0; --p)
@@ -677,6 +687,7 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
       const float eC = now.eC;
       load(c + 2, now);
       lds_barrier();
+      if constexpr (DELTA) __builtin_amdgcn_s_setprio(3);
       uint4 uf[3][2];
 #pragma unroll
       for (int p = 2; p >= 0; --p)
@@ -726,8 +737,8 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
   if (wave >= 8) {
     // ------------------------------------------------------- output waves
     u32x4 p[4];
+    uint4 qf[KS];
     f32x4 eG, qs;
-    uint4 u[UP][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[j] = (u32x4){0, 0, 0, 0};  // above the diagonal: stay zero
     auto load = [&](int c) {
@@ -738,18 +749,37 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
       for (int j = 0; j < 4; ++j)
         if (j <= w4) p[j] = *reinterpret_cast<const u32x4*>(m + j * kStep + l16);
     };
-    auto take = [&](int b) {
-      f32x4 q[KS];
+    auto load_q = [&](int c) {
+      const char* m = static_cast<const char*>(a.workspace) + a.key_offset +
+                      ((c0 + clamped(c)) * a.k_heads + hk) * (int64_t)KeyData<DK>::bytes +
+                      KeyData<DK>::q + w4 * kStep;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) q[s] = Qp[b][s][w4][lane];
+      for (int s = 0; s < KS; ++s) qf[s] = load16(m + s * 4 * kStep + l16);
+    };
+    auto q_times_state = [&] {
+      uint4 sf[2][KS];
 #pragma unroll
-      for (int e = 0; e < UP; ++e) u[e][0] = Uf[b][e][0][lane], u[e][1] = Uf[b][e][1][lane];
-      qs = q[0] + q[1];
-      if constexpr (KS == 4) qs += q[2] + q[3];
+      for (int s = 0; s < KS; ++s) sf[0][s] = Sf[0][s][lane], sf[1][s] = Sf[1][s][lane];
+      f32x4 q0 = {0.0f, 0.0f, 0.0f, 0.0f}, q1 = q0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        q0 = mfma(frag(qf[s]), frag(sf[0][s]), q0);
+        q1 = mfma(frag(qf[s]), frag(sf[1][s]), q1);
+      }
+      qs = q0 + q1;
     };
     // scale (e^G q S + P U)
-    const int64_t o_row = (int64_t)a.v_heads * a.dv;
-    auto finish = [&](int c) {
+    uint16_t o16[4];
+    auto compute = [&](int b) {
+      uint4 u[UP][2];
+#pragma unroll
+      for (int e = 0; e < UP; ++e) u[e][0] = Uf[b][e][0][lane], u[e][1] = Uf[b][e][1][lane];
+      f32x4 part[DELTA ? 1 : KS];
+      if constexpr (!DELTA) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) part[s] = Qp[b][s][w4][lane];
+      }
+      issue_fence();
       f32x4 o0 = {0.0f, 0.0f, 0.0f, 0.0f}, o1 = o0, o2 = o0;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -760,7 +790,16 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
         o1 = mfma(frag(make_uint4(l.z, l.w, r.z, r.w)), frag(u[0][ks]), o1);
         if constexpr (DELTA) o2 = mfma(p0, frag(u[UP - 1][ks]), o2);
       }
+      if constexpr (!DELTA) {
+        qs = part[0] + part[1];
+        if constexpr (KS == 4) qs += part[2] + part[3];
+      }
       const f32x4 o = a.scale * (eG * qs + (o0 + (o1 + o2)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o16[i] = (uint16_t)f32_to_bf16(o[i]);
+    };
+    const int64_t o_row = (int64_t)a.v_heads * a.dv;
+    auto store = [&](int c) {
       char* base = reinterpret_cast<char*>(
           a.out + (sq.begin + (int64_t)c * kChunk) * o_row + (int64_t)hv * a.dv);
       const int left = sq.len - c * kChunk;
@@ -768,25 +807,32 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
       for (int i = 0; i < 4; ++i)
         if (i0 + i < left)
           *reinterpret_cast<uint16_t*>(
-              base + ((uint32_t)(i0 + i) * ((uint32_t)o_row * 2u) + 2u * (uint32_t)col)) =
-              (uint16_t)f32_to_bf16(o[i]);
-      load(c + 1);
+              base + ((uint32_t)(i0 + i) * ((uint32_t)o_row * 2u) + 2u * (uint32_t)col)) = o16[i];
     };
+    // q S between a chunk's second and third exchange, P U between its third
+    // and the next one's first, stores and loads behind that: no exchange
+    // waits for an output wave.
     load(0);
+    if constexpr (DELTA) load_q(0);
     for (int c = 0; c < chunks; ++c) {
+      lds_barrier();
       if constexpr (DELTA) {
+        if (c > 0) {
+          store(c - 1);
+          load(c);
+        }
         lds_barrier();
+        q_times_state();
+        load_q(c + 1);
         lds_barrier();
-        if (c > 0) finish(c - 1);
-        lds_barrier();
-        take(0);
+        compute(0);
       } else {
-        lds_barrier();
-        take(c & 1);
-        finish(c);
+        compute(c & 1);
+        store(c);
+        load(c + 1);
       }
     }
-    if constexpr (DELTA) finish(chunks - 1);
+    if constexpr (DELTA) store(chunks - 1);
     return;
   }
 
@@ -835,6 +881,7 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
     f32x4 u;
     if constexpr (DELTA) {
       lds_barrier();
+      __builtin_amdgcn_s_setprio(3);
       f32x4 k[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) k[s] = Kp[s][w4][lane];
@@ -878,6 +925,7 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
     }
     put_u(b, u, x.dec);
     lds_barrier();
+    __builtin_amdgcn_s_setprio(0);
     load(c + 2, x);
   };
   Loads even, odd;

@@ -130,10 +130,11 @@ __device__ __forceinline__ float sum_over_rows(float v) {
 // A wave holds 4 LC columns of a state: lane (rg, c) the rows rg RW .. of
 // columns 4 c .. 4 c + 3.  Both sums over the rows, S^T k and S^T q, are of
 // the state before the token, so a token costs one round of exchanges:
-// o = a S^T q + (q.k) u.  Bound by the state's read and write; LC 8 moves
-// whole lines (127 tokens x 32 heads of 128 x 128: 106 us, 5.0 TB/s, against
-// 121 with LC 4 and 108 with 16), LC 4 has twice the waves for few states (one
-// token x 32 heads: 5.0 us against 5.6).
+// o = a S^T q + (q.k) u.  Bound by the state's read and write: 127 tokens x 32
+// heads of 128 x 128 101 us, 5.3 TB/s.  LC 8 moves whole lines (there 106 us
+// before the next token was loaded ahead, against 121 with LC 4 and 108 with
+// 16), LC 4 has twice the waves for few states (one token x 32 heads: 4.4 us,
+// 5.6 with LC 8).
 template <int DK, bool DELTA, int LC>
 __device__ __forceinline__ void by_token(const LinearArgs& a, int64_t group) {
   constexpr int RW = DK * LC / kWave;  // rows of a lane
@@ -529,7 +530,7 @@ __global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const Li
   clear_uncovered(a, (int)(block - chunks), kClearParts);
 }
 
-// One (sequence, head, 16 columns of the state) from chunk to chunk, twelve
+// One (sequence, head, 16 NT columns of the state) from chunk to chunk, twelve
 // waves, three to a SIMD (one alone waits between its instructions):
 //
 //   - state waves 0 to 3 hold 32 dims of the state each and multiply them, as
@@ -537,27 +538,27 @@ __global__ __launch_bounds__(kLinThreads, 5) void linear_prepare_kernel(const Li
 //     accumulator's lane holds rows 4 g + i of its column, four of the eight
 //     contraction indices that the same lane needs in operand B;
 //   - token waves 4 to 7 take 16 tokens each, add up the partial K S and make U;
-//   - output waves 8 to 11 take 16 tokens each and make the outputs of the chunk
-//     before.
+//   - output waves 8 to 11 take 16 tokens each and make q S and, when U is
+//     there, the outputs, while the others are in the next chunk.
 //
 // With the delta rule a chunk is a chain of three exchanges through LDS
 // (partial K S, the residual, U) between the first two; what is not in the
 // chain (outputs, q S, turning k, loads) is done by whoever is not in it.
 // Without it U is v, and one exchange is left.
-template <int DK, bool DELTA>
+template <int DK, bool DELTA, int NT>
 __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int hv, int tile) {
   constexpr int KS = DK / 32;         // state waves
   constexpr int SP = DELTA ? 3 : 2;   // pieces of the state that a product takes
   constexpr int UP = DELTA ? 2 : 1;   // of U in P U (v alone is bf16 as it is)
   constexpr int BUF = DELTA ? 1 : 2;  // one exchange a chunk: two buffers in turn
-  __shared__ f32x4 Kp[DELTA ? KS : 1][4][kWave];  // partial K S of each 16 tokens
+  __shared__ f32x4 Kp[DELTA ? KS : 1][4 * NT][kWave];  // partial K S of each 16 tokens
   // q S: of the output waves, from two pieces of the state; without beta, where
   // they are the busiest, of the state waves, in parts
-  __shared__ uint4 Sf[2][KS][kWave];
-  __shared__ f32x4 Qp[BUF][DELTA ? 1 : KS][4][kWave];
-  __shared__ uint4 Rf[DELTA ? 3 : 1][2][kWave];
-  __shared__ uint4 Uf[BUF][UP + 3][2][kWave];
-  __shared__ uint4 Kt[KS][4][kWave];              // a state wave's dims of k, to be transposed
+  __shared__ uint4 Sf[2][KS][NT][kWave];
+  __shared__ f32x4 Qp[BUF][DELTA ? 1 : KS][4 * NT][kWave];
+  __shared__ uint4 Rf[DELTA ? 3 : 1][2][NT][kWave];
+  __shared__ uint4 Uf[BUF][UP + 3][2][NT][kWave];
+  __shared__ uint4 Kt[KS][4][kWave];  // a state wave's dims of k, to be transposed
 
   const int hk = hv / (a.v_heads / a.k_heads);
   const Seq sq = seq_of(a, r);
@@ -567,16 +568,17 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w4 = wave & 3;  // its dims 32 w4 .. or its tokens 16 w4 ..
   const int n = lane & 15, g = lane >> 4;
-  const int col = tile * 16 + n;
+  const int col = tile * (16 * NT) + n;  // and every 16th on
   const int chunks = (sq.len + kChunk - 1) / kChunk;
   const int64_t c0 = chunk_base(a, r);
   const char* ws0 = static_cast<const char*>(a.workspace) +
                     (c0 * a.v_heads + hv) * (int64_t)ChunkData<DELTA>::bytes;
   const int64_t ws_step = (int64_t)a.v_heads * ChunkData<DELTA>::bytes;
   const uint32_t l16 = lane * 16;
-  // Operands are loaded two chunks ahead, into two sets used in turn, by each
-  // kind of wave while the chain is with the other kind; past the end the last
-  // chunk's are loaded again, which needs no branch.
+  // State and token waves load their operands two chunks ahead, into two sets
+  // used in turn, each kind while the chain is with the other; output waves,
+  // which have time, one chunk ahead.  Past the end the last chunk's are loaded
+  // again, which needs no branch.
   auto clamped = [&](int c) { return c < chunks ? c : chunks - 1; };
 
   if (wave < 4) {
@@ -591,14 +593,16 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
       }
       return;
     }
-    // lane (g, n) of tile h: dims 32 w4 + 8 g + 4 h + i of column n
-    f32x4 S[2];
+    // lane (g, n) of tile h: dims 32 w4 + 8 g + 4 h + i of column 16 nt + n
+    f32x4 S[NT][2];
     const int64_t at = ((slot * a.v_heads + hv) * DK + 32 * w4 + 8 * g) * a.dv + col;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        S[h][i] = slot >= 0 ? a.state[at + (int64_t)(4 * h + i) * a.dv] : 0.0f;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          S[nt][h][i] = slot >= 0 ? a.state[at + (int64_t)(4 * h + i) * a.dv + 16 * nt] : 0.0f;
 
     const char* key0 = static_cast<const char*>(a.workspace) + a.key_offset +
                        (c0 * a.k_heads + hk) * (int64_t)KeyData<DK>::bytes + w4 * 4 * kStep;
@@ -648,63 +652,77 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
     };
     auto step = [&](int c, Loads& now) {
       const int b = DELTA ? 0 : c & 1;
-      uint32_t lo[SP][2], up[SP][2];
-      pieces<SP>(S[0], lo);
-      pieces<SP>(S[1], up);
-      bf16x8 sf[SP];
+      bf16x8 sf[NT][SP];
 #pragma unroll
-      for (int p = 0; p < SP; ++p) {
-        const uint32_t w[4] = {lo[p][0], lo[p][1], up[p][0], up[p][1]};
-        sf[p] = frag(w);
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t lo[SP][2], up[SP][2];
+        pieces<SP>(S[nt][0], lo);
+        pieces<SP>(S[nt][1], up);
+#pragma unroll
+        for (int p = 0; p < SP; ++p) {
+          const uint32_t w[4] = {lo[p][0], lo[p][1], up[p][0], up[p][1]};
+          sf[nt][p] = frag(w);
+        }
       }
       if constexpr (DELTA) {
-        f32x4 x[4] = {};
+        f32x4 x[4 * NT] = {};
 #pragma unroll
         for (int p = SP - 1; p >= 0; --p)  // from the least up
 #pragma unroll
-          for (int t = 0; t < 4; ++t) x[t] = mfma(frag(now.k[t]), sf[p], x[t]);
+          for (int t = 0; t < 4 * NT; ++t)
+            x[t] = mfma(frag(now.k[t / NT]), sf[t % NT][p], x[t]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) Kp[w4][t][lane] = x[t];
+        for (int t = 0; t < 4 * NT; ++t) Kp[w4][t][lane] = x[t];
         lds_barrier();
         __builtin_amdgcn_s_setprio(0);  // out of the chain until U is there
       }
       bf16x8 kt[2][2];
       if constexpr (DELTA) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) *reinterpret_cast<bf16x8*>(&Sf[p][w4][lane]) = sf[p];
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            *reinterpret_cast<bf16x8*>(&Sf[p][w4][nt][lane]) = sf[nt][p];
         lds_barrier();
         transpose(now, kt);
       } else {
         transpose(now, kt);
-        f32x4 x[4] = {};
+        f32x4 x[4 * NT] = {};
 #pragma unroll
         for (int p = 1; p >= 0; --p)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) x[t] = mfma(frag(now.q[t]), sf[p], x[t]);
+          for (int t = 0; t < 4 * NT; ++t)
+            x[t] = mfma(frag(now.q[t / NT]), sf[t % NT][p], x[t]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) Qp[b][w4][t][lane] = x[t];
+        for (int t = 0; t < 4 * NT; ++t) Qp[b][w4][t][lane] = x[t];
       }
       const float eC = now.eC;
       load(c + 2, now);
       lds_barrier();
       if constexpr (DELTA) __builtin_amdgcn_s_setprio(3);
-      uint4 uf[3][2];
+      uint4 uf[NT][3][2];
 #pragma unroll
       for (int p = 2; p >= 0; --p)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) uf[p][ks] = Uf[b][UP + p][ks][lane];
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) uf[nt][p][ks] = Uf[b][UP + p][ks][nt][lane];
       issue_fence();
-      f32x4 y[2][2] = {};
+      f32x4 y[NT][2][2] = {};
 #pragma unroll
       for (int p = 2; p >= 0; --p)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            y[h][ks] = mfma(kt[h][ks], frag(uf[p][ks]), y[h][ks]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              y[nt][h][ks] = mfma(kt[h][ks], frag(uf[nt][p][ks]), y[nt][h][ks]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) S[h] = eC * S[h] + (y[h][0] + y[h][1]);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) S[nt][h] = eC * S[nt][h] + (y[nt][h][0] + y[nt][h][1]);
     };
     if (chunks > 0) {
       Loads even, odd;
@@ -719,9 +737,12 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
     }
     if (slot < 0) return;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a.state_out[at + (int64_t)(4 * h + i) * a.dv] = S[h][i];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          a.state_out[at + (int64_t)(4 * h + i) * a.dv + 16 * nt] = S[nt][h][i];
     return;
   }
 
@@ -738,7 +759,7 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
     // ------------------------------------------------------- output waves
     u32x4 p[4];
     uint4 qf[KS];
-    f32x4 eG, qs;
+    f32x4 eG, qs[NT];
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[j] = (u32x4){0, 0, 0, 0};  // above the diagonal: stay zero
     auto load = [&](int c) {
@@ -757,27 +778,30 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
       for (int s = 0; s < KS; ++s) qf[s] = load16(m + s * 4 * kStep + l16);
     };
     auto q_times_state = [&] {
-      uint4 sf[2][KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) sf[0][s] = Sf[0][s][lane], sf[1][s] = Sf[1][s][lane];
-      f32x4 q0 = {0.0f, 0.0f, 0.0f, 0.0f}, q1 = q0;
+      for (int nt = 0; nt < NT; ++nt) {
+        uint4 sf[2][KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        q0 = mfma(frag(qf[s]), frag(sf[0][s]), q0);
-        q1 = mfma(frag(qf[s]), frag(sf[1][s]), q1);
+        for (int s = 0; s < KS; ++s) sf[0][s] = Sf[0][s][nt][lane], sf[1][s] = Sf[1][s][nt][lane];
+        f32x4 q0 = {0.0f, 0.0f, 0.0f, 0.0f}, q1 = q0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          q0 = mfma(frag(qf[s]), frag(sf[0][s]), q0);
+          q1 = mfma(frag(qf[s]), frag(sf[1][s]), q1);
+        }
+        qs[nt] = q0 + q1;
       }
-      qs = q0 + q1;
     };
     // scale (e^G q S + P U)
-    uint16_t o16[4];
-    auto compute = [&](int b) {
+    uint16_t o16[NT][4];
+    auto compute = [&](int b, int nt) {
       uint4 u[UP][2];
 #pragma unroll
-      for (int e = 0; e < UP; ++e) u[e][0] = Uf[b][e][0][lane], u[e][1] = Uf[b][e][1][lane];
+      for (int e = 0; e < UP; ++e) u[e][0] = Uf[b][e][0][nt][lane], u[e][1] = Uf[b][e][1][nt][lane];
       f32x4 part[DELTA ? 1 : KS];
       if constexpr (!DELTA) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) part[s] = Qp[b][s][w4][lane];
+        for (int s = 0; s < KS; ++s) part[s] = Qp[b][s][w4 * NT + nt][lane];
       }
       issue_fence();
       f32x4 o0 = {0.0f, 0.0f, 0.0f, 0.0f}, o1 = o0, o2 = o0;
@@ -791,12 +815,16 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
         if constexpr (DELTA) o2 = mfma(p0, frag(u[UP - 1][ks]), o2);
       }
       if constexpr (!DELTA) {
-        qs = part[0] + part[1];
-        if constexpr (KS == 4) qs += part[2] + part[3];
+        qs[nt] = part[0] + part[1];
+        if constexpr (KS == 4) qs[nt] += part[2] + part[3];
       }
-      const f32x4 o = a.scale * (eG * qs + (o0 + (o1 + o2)));
+      const f32x4 o = a.scale * (eG * qs[nt] + (o0 + (o1 + o2)));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o16[i] = (uint16_t)f32_to_bf16(o[i]);
+      for (int i = 0; i < 4; ++i) o16[nt][i] = (uint16_t)f32_to_bf16(o[i]);
+    };
+    auto compute_all = [&](int b) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) compute(b, nt);
     };
     const int64_t o_row = (int64_t)a.v_heads * a.dv;
     auto store = [&](int c) {
@@ -805,9 +833,12 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
       const int left = sq.len - c * kChunk;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i0 + i < left)
-          *reinterpret_cast<uint16_t*>(
-              base + ((uint32_t)(i0 + i) * ((uint32_t)o_row * 2u) + 2u * (uint32_t)col)) = o16[i];
+        if (i0 + i < left) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            *reinterpret_cast<uint16_t*>(base + ((uint32_t)(i0 + i) * ((uint32_t)o_row * 2u) +
+                                                 2u * (uint32_t)(col + 16 * nt))) = o16[nt][i];
+        }
     };
     // q S between a chunk's second and third exchange, P U between its third
     // and the next one's first, stores and loads behind that: no exchange
@@ -825,9 +856,9 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
         q_times_state();
         load_q(c + 1);
         lds_barrier();
-        compute(0);
+        compute_all(0);
       } else {
-        compute(c & 1);
+        compute_all(c & 1);
         store(c);
         load(c + 1);
       }
@@ -840,7 +871,7 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
   struct Loads {
     u32x4 t01[DELTA ? 4 : 1];
     u32x2 t2[DELTA ? 4 : 1];
-    uint16_t v[4];
+    uint16_t v[NT][4];
     f32x4 eG, dec;
   };
   auto load = [&](int c, Loads& x) {
@@ -862,68 +893,82 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
         a.v + (sq.begin + (int64_t)c * kChunk) * a.v_row + hv * a.v_head);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      x.v[e] = *reinterpret_cast<const uint16_t*>(
-          base + ((uint32_t)min(i0 + e, last) * ((uint32_t)a.v_row * 2u) + 2u * (uint32_t)col));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        x.v[nt][e] = *reinterpret_cast<const uint16_t*>(
+            base + ((uint32_t)min(i0 + e, last) * ((uint32_t)a.v_row * 2u) +
+                    2u * (uint32_t)(col + 16 * nt)));
   };
-  auto put_u = [&](int b, const f32x4 u, const f32x4 dec) {
+  auto put_u = [&](int b, int nt, const f32x4 u, const f32x4 dec) {
     uint32_t w[UP][2], y[3][2];
     pieces<3>(dec * u, y);
 #pragma unroll
     for (int p = 0; p < 3; ++p)
-      reinterpret_cast<uint2*>(&Uf[b][UP + p][w4 >> 1][lane])[w4 & 1] = make_uint2(y[p][0], y[p][1]);
+      reinterpret_cast<uint2*>(&Uf[b][UP + p][w4 >> 1][nt][lane])[w4 & 1] = make_uint2(y[p][0], y[p][1]);
     pieces<UP>(u, w);
 #pragma unroll
     for (int p = 0; p < UP; ++p)
-      reinterpret_cast<uint2*>(&Uf[b][p][w4 >> 1][lane])[w4 & 1] = make_uint2(w[p][0], w[p][1]);
+      reinterpret_cast<uint2*>(&Uf[b][p][w4 >> 1][nt][lane])[w4 & 1] = make_uint2(w[p][0], w[p][1]);
   };
   auto step = [&](int c, Loads& x) {
     const int b = DELTA ? 0 : c & 1;
-    f32x4 u;
+    f32x4 u[NT];
     if constexpr (DELTA) {
       lds_barrier();
       __builtin_amdgcn_s_setprio(3);
-      f32x4 k[KS];
+      f32x4 k[NT][KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) k[s] = Kp[s][w4][lane];
-      f32x4 ks = k[0] + k[1];
-      if constexpr (KS == 4) ks += k[2] + k[3];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = bf16_to_f32(x.v[i]) - x.eG[i] * ks[i];
-      uint32_t w[3][2];
-      pieces<3>(u, w);
+        for (int s = 0; s < KS; ++s) k[nt][s] = Kp[s][w4 * NT + nt][lane];
 #pragma unroll
-      for (int p = 0; p < 3; ++p)
-        reinterpret_cast<uint2*>(&Rf[p][w4 >> 1][lane])[w4 & 1] = make_uint2(w[p][0], w[p][1]);
-      lds_barrier();
-      uint4 rf[3][2];
+      for (int nt = 0; nt < NT; ++nt) {
+        f32x4 ks = k[nt][0] + k[nt][1];
+        if constexpr (KS == 4) ks += k[nt][2] + k[nt][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < 4; ++i) u[nt][i] = bf16_to_f32(x.v[nt][i]) - x.eG[i] * ks[i];
+        uint32_t w[3][2];
+        pieces<3>(u[nt], w);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) rf[p][s] = Rf[p][s][lane];
-      issue_fence();
-      // six chains of one or two products; the sum goes from the least up
-      f32x4 y[6] = {};
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s && !two) continue;
-        const u32x4 l = x.t01[2 * s], r = x.t01[2 * s + 1];
-        const u32x2 l2 = x.t2[2 * s], r2 = x.t2[2 * s + 1];
-        const bf16x8 t0 = frag(make_uint4(l.x, l.y, r.x, r.y));
-        const bf16x8 t1 = frag(make_uint4(l.z, l.w, r.z, r.w));
-        const bf16x8 t2 = frag(make_uint4(l2.x, l2.y, r2.x, r2.y));
-        y[0] = mfma(t0, frag(rf[0][s]), y[0]);
-        y[1] = mfma(t0, frag(rf[1][s]), y[1]);
-        y[2] = mfma(t1, frag(rf[0][s]), y[2]);
-        y[3] = mfma(t0, frag(rf[2][s]), y[3]);
-        y[4] = mfma(t1, frag(rf[1][s]), y[4]);
-        y[5] = mfma(t2, frag(rf[0][s]), y[5]);
+        for (int p = 0; p < 3; ++p)
+          reinterpret_cast<uint2*>(&Rf[p][w4 >> 1][nt][lane])[w4 & 1] = make_uint2(w[p][0], w[p][1]);
       }
-      u = y[0] + ((y[1] + y[2]) + (y[3] + (y[4] + y[5])));
+      lds_barrier();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint4 rf[3][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) rf[p][s] = Rf[p][s][nt][lane];
+        issue_fence();
+        // six chains of one or two products; the sum goes from the least up
+        f32x4 y[6] = {};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s && !two) continue;
+          const u32x4 l = x.t01[2 * s], r = x.t01[2 * s + 1];
+          const u32x2 l2 = x.t2[2 * s], r2 = x.t2[2 * s + 1];
+          const bf16x8 t0 = frag(make_uint4(l.x, l.y, r.x, r.y));
+          const bf16x8 t1 = frag(make_uint4(l.z, l.w, r.z, r.w));
+          const bf16x8 t2 = frag(make_uint4(l2.x, l2.y, r2.x, r2.y));
+          y[0] = mfma(t0, frag(rf[0][s]), y[0]);
+          y[1] = mfma(t0, frag(rf[1][s]), y[1]);
+          y[2] = mfma(t1, frag(rf[0][s]), y[2]);
+          y[3] = mfma(t0, frag(rf[2][s]), y[3]);
+          y[4] = mfma(t1, frag(rf[1][s]), y[4]);
+          y[5] = mfma(t2, frag(rf[0][s]), y[5]);
+        }
+        u[nt] = y[0] + ((y[1] + y[2]) + (y[3] + (y[4] + y[5])));
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = bf16_to_f32(x.v[i]);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[nt][i] = bf16_to_f32(x.v[nt][i]);
     }
-    put_u(b, u, x.dec);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) put_u(b, nt, u[nt], x.dec);
     lds_barrier();
     __builtin_amdgcn_s_setprio(0);
     load(c + 2, x);
@@ -948,42 +993,73 @@ __device__ __forceinline__ void through_chunks(const LinearArgs& a, int r, int h
 
 // The column tiles of a head on one XCD, whose L2 then holds the head's chunk,
 // and with enough of them the heads that share q and k.
-__host__ __device__ __forceinline__ int64_t chunk_items(const LinearArgs& a, int64_t sequences) {
+__host__ __device__ __forceinline__ int64_t chunk_items(const LinearArgs& a, int64_t sequences,
+                                                        int nt) {
   const int64_t units = sequences * a.v_heads / a.span;
-  return (units + 7) / 8 * 8 * a.span * (a.dv / 16);
+  return (units + 7) / 8 * 8 * a.span * (a.dv / (16 * nt));
 }
 
-template <int DK, bool DELTA>
+template <int DK, bool DELTA, int NT>
 __device__ __forceinline__ void chunk_item(const LinearArgs& a, int64_t id, int count) {
-  const int tiles = a.dv / 16;
+  const int tiles = a.dv / (16 * NT);
   const int64_t in_xcd = id >> 3;
   const int64_t at_xcd = in_xcd / tiles;
   const int64_t head = (at_xcd / a.span * 8 + (id & 7)) * a.span + at_xcd % a.span;
   if (head >= (int64_t)count * a.v_heads) return;
   const int which = (int)(head / a.v_heads);
-  through_chunks<DK, DELTA>(a, a.list ? a.list[1 + which] : 0,
-                            (int)(head - (int64_t)which * a.v_heads), (int)(in_xcd % tiles));
+  through_chunks<DK, DELTA, NT>(a, a.list ? a.list[1 + which] : 0,
+                                (int)(head - (int64_t)which * a.v_heads), (int)(in_xcd % tiles));
+}
+
+// Workgroups of listed sequences' chunks: one a compute unit is all that the
+// registers allow, and a workgroup without work would cost a turn.
+constexpr int64_t kChunkGroups = 256;
+
+// Whether an item takes 32 columns: its chain has waits that a second tile
+// fills, and its operands are read once for both, so that two tiles take about
+// 1.4 times one's time.  That pays where it saves more than a third of the
+// rounds (32 heads of 128 x 128, with the delta rule and without: 4 sequences
+// of 8192 tokens 1015 -> 781 and 721 -> 677 us, 16 of 512 303 -> 248 and
+// 215 -> 189; 3 of 2048, three rounds against two, 183 -> 184 and 121 -> 135).
+__host__ __device__ __forceinline__ bool two_tiles(const LinearArgs& a, int64_t sequences) {
+  if (a.dv % 32) return false;
+  const int64_t one = (chunk_items(a, sequences, 1) + kChunkGroups - 1) / kChunkGroups;
+  const int64_t two = (chunk_items(a, sequences, 2) + kChunkGroups - 1) / kChunkGroups;
+  return 3 * two < 2 * one;
 }
 
 // A workgroup takes one item of the only sequence, or of listed ones its item
-// and those a grid further on, which are on the same XCD.  (The loop costs the
-// chunks 8% of their time in registers: 8192 tokens x 32 heads 230 us for 213.)
-template <int DK, bool DELTA, bool LISTED>
-__global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const LinearArgs a) {
+// and those a grid further on, which are on the same XCD.  Only the list knows
+// how many there are: where that could call for either width both kernels are
+// launched, and one of them ends at once (2 us; with both in one kernel the
+// registers spill, which costs 4 to 30%).
+template <int DK, bool DELTA, int NT, bool LISTED>
+__global__ __launch_bounds__(kChunkThreads) void linear_chunk_kernel(const LinearArgs a,
+                                                                     bool either) {
   if constexpr (!LISTED) {
-    chunk_item<DK, DELTA>(a, blockIdx.x, 1);
+    chunk_item<DK, DELTA, NT>(a, blockIdx.x, 1);
   } else {
     const int count = a.list[0];
-    const int64_t items = chunk_items(a, count);
+    if (either && two_tiles(a, count) != (NT == 2)) return;
+    const int64_t items = chunk_items(a, count, NT);
     for (int64_t id = blockIdx.x; id < items; id += gridDim.x) {
-      chunk_item<DK, DELTA>(a, id, count);
+      chunk_item<DK, DELTA, NT>(a, id, count);
       lds_barrier();  // the next one's first exchange writes where this one's last is read
     }
   }
 }
-// Workgroups of the chunk kernel: one a compute unit is all that its registers
-// allow, and a workgroup without work would cost a turn.
-constexpr int64_t kChunkGroups = 256;
+
+template <int DK, bool DELTA, int NT>
+hipError_t launch_chunks(const LinearArgs& a, int64_t sequences, bool either, hipStream_t s) {
+  const int64_t items = chunk_items(a, sequences, NT);
+  if (!a.list)
+    linear_chunk_kernel<DK, DELTA, NT, false><<<(unsigned)items, kChunkThreads, 0, s>>>(a, false);
+  else
+    linear_chunk_kernel<DK, DELTA, NT, true>
+        <<<(unsigned)(items < kChunkGroups ? items : kChunkGroups), kChunkThreads, 0, s>>>(a,
+                                                                                          either);
+  return hipGetLastError();
+}
 
 template <int DK, bool DELTA>
 hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
@@ -1000,18 +1076,14 @@ hipError_t launch_linear_of(const LinearArgs& a, hipStream_t s) {
   const int64_t beside = a.list ? 1 + token_groups(a, 4) : 0;
   linear_prepare_kernel<DK, DELTA>
       <<<(unsigned)(beside + a.chunks * a.v_heads + clear), kLinThreads, 0, s>>>(a);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (!a.list) {
-    linear_chunk_kernel<DK, DELTA, false>
-        <<<(unsigned)chunk_items(a, 1), kChunkThreads, 0, s>>>(a);
-    return hipGetLastError();
-  }
   const int64_t most = a.tokens / (a.by_token + 1);  // sequences that go in chunks
-  const int64_t items = chunk_items(a, most < a.requests ? most : a.requests);
-  linear_chunk_kernel<DK, DELTA, true>
-      <<<(unsigned)(items < kChunkGroups ? items : kChunkGroups), kChunkThreads, 0, s>>>(a);
-  return hipGetLastError();
+  const int64_t sequences = !a.list ? 1 : most < a.requests ? most : a.requests;
+  const bool two = two_tiles(a, sequences);
+  if (two) e = launch_chunks<DK, DELTA, 2>(a, sequences, true, s);
+  if (e != hipSuccess || (two && !a.list)) return e;
+  return launch_chunks<DK, DELTA, 1>(a, sequences, two, s);
 }
 
 }  // namespace

@@ -459,6 +459,17 @@ def test_linear_mixed(native, R, delta):
 
 
 @pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("lens", [[131], [70, 130, 26, 66], [65, 30, 3, 129]])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_linear_many_states(native, lens, dk, delta):
+    """More states than the chip takes at once, which go through the chunks by
+    32 columns: one sequence, several, and several of which one turns out to
+    be short, so that by 16 saves a round."""
+    vh = 64 if len(lens) == 1 else 32
+    check_linear(native, *linear_inputs(dk, lens, 8, vh, dk, 128, delta))
+
+
+@pytest.mark.parametrize("delta", [True, False])
 @pytest.mark.parametrize("decay", [0.0, -1e-4, -0.3, -40.0, -float("inf")])
 def test_linear_decays(native, decay, delta):
     """One rate for a head, expanded over the tokens: none, slow, and so

@@ -340,7 +340,9 @@ int rmoe_stream_read(const void* buffer, size_t bytes, uint32_t* partials,
  * version 7).  No counterpart in the reference, whose attention and linear
  * attention are mlx-lm's; the layers are those of docs/architecture.md:31-37.
  * The calls below keep no counters: their workspaces need no zero-fill and
- * hold nothing between calls. */
+ * hold nothing between calls.  A call's outputs and its workspace lie apart
+ * from its inputs and from each other, except where an input is said to be
+ * written in place. */
 
 /* Rows of heads: value d of head h of row t is x[t * row_stride + h *
  * head_stride + d], bf16; x 16-byte aligned, strides multiples of 8. */
@@ -411,8 +413,7 @@ int rmoe_paged_tables(const int32_t* cached, const int32_t* added, int32_t reque
 /* Rotary positions: q_out [rows, q heads, dim] and k_out [rows, k heads, dim]
  * = the turned rows (angles in 64 bits, products fp32, one rounding), values
  * past 2 * half copied.  positions int32, axis a's at positions + a *
- * axis_stride.  dim a multiple of 8, at most 1024.  Outputs must not overlap
- * inputs. */
+ * axis_stride.  dim a multiple of 8, at most 1024. */
 int rmoe_rotary(const rmoe_rotary_spec* spec, const int32_t* positions, int64_t axis_stride,
                 int32_t rows, int32_t dim, const rmoe_rows* q, uint16_t* q_out,
                 const rmoe_rows* k, uint16_t* k_out, void* stream);

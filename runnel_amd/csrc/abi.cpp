@@ -1202,8 +1202,9 @@ int rmoe_paged_attention(const rmoe_rows* q, const rmoe_paged_cache* cache,
                          void* stream) {
   int rc;
   if ((rc = check_cache(cache))) return rc;
-  if (requests < 0 || table_width < 0 || window < 0)
-    return fail(RMOE_EINVAL, "requests, table_width and window must not be negative");
+  if (requests < 0 || table_width < 0 || table_stride < 0 || window < 0)
+    return fail(RMOE_EINVAL,
+                "requests, table_width, table_stride and window must not be negative");
   if ((rc = check_rows_of(q, "q", requests > 0))) return rc;
   if (q->heads % cache->kv_heads)
     return fail(RMOE_EINVAL, "query heads must be a multiple of the %d key heads (got %d)",

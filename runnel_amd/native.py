@@ -896,6 +896,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     cache = _cache(k_cache, v_cache, k_scale, v_scale)
     if 0 in k_cache.stride():
         raise ValueError("an expanded cache cannot be written")
+    if cache.k == cache.v:
+        raise ValueError("k_cache and v_cache must be two")
     q, qr = _heads(q, "q", None, None, cache.dim)
     N = q.shape[0]
     k, kr = _heads(k, "k", N, cache.kv_heads, cache.dim)

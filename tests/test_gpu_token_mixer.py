@@ -251,6 +251,15 @@ def test_append_special_values(native):
         assert torch.equal(tail.isnan(), want[16:].isnan())
 
 
+def test_append_refuses_one_cache(native):
+    """Keys and values into one place: either could be left there."""
+    x, c = torch.zeros(1, 1, 64, dtype=BF16, device="cuda"), torch.zeros(1, 1, 8, 64, dtype=BF16, device="cuda")
+    i = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for k, v, why in ((c, c.view(1, 1, 8, 64), "must be two"), (c.expand(4, 1, 8, 64), c.expand(4, 1, 8, 64), "expanded")):
+        with pytest.raises(ValueError, match=why):
+            native.rotary_append(x, x, x, i, torch.zeros(8, device="cuda"), k, v, i.long())
+
+
 # ---------------------------------------------------------------- attention
 
 
@@ -358,6 +367,38 @@ def test_attention_bad_pages(native):
     # no table at all
     none = native.paged_attention(q.cuda(), kc, vc, table.cuda()[:, :0], lengths.cuda())
     assert bool((none == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_cache_past_32_bits(native, dtype):
+    """Pages whose values lie more than 2^31 values (bf16: 2^32 bytes) into
+    the cache, written and read; the pages between are nobody's."""
+    pages, page, D = 32800, 1024, 64
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 9 GB of the GPU's memory")
+    kc, vc = (torch.empty((pages, 1, page, D), dtype=dtype, device="cuda") for _ in range(2))
+    ids = [pages - 1, 3, pages - 2]
+    for c in (kc, vc):
+        raw(c)[ids] = 0
+    g = gen(3)
+    N = 2 * page + 100
+    x = randn(g, N, 3, D).to(BF16).cuda()
+    table = torch.tensor([ids], dtype=torch.int32, device="cuda")
+    t = native.paged_tables(torch.zeros(1, dtype=torch.int32, device="cuda"),
+                            torch.tensor([N], dtype=torch.int32, device="cuda"), table.clone(),
+                            table[0], page, N)
+    inv = torch.zeros(8, device="cuda")
+    q = native.rotary_append(x[:, :1], x[:, 1:2], x[:, 2:], t.positions, inv, kc, vc, t.slots)
+    small = [c[torch.tensor(ids, device="cuda")] if dtype == BF16 else raw(c)[ids].view(dtype) for c in (kc, vc)]
+    want = x[:, 1:].to(dtype).cpu().float()
+    for i in range(2):
+        flat = small[i].cpu().float().reshape(-1, D)
+        assert torch.equal(flat[:N], want[:, i]) and bool((flat[N:] == 0).all())
+    last = q[-1:].cpu()
+    near = torch.tensor([[0, 1, 2]], dtype=torch.int32)
+    ref = check_attention(native, last, *small, near, t.lengths.cpu())
+    got = native.paged_attention(last.cuda(), kc, vc, table, t.lengths)
+    assert torch.equal(got, ref)  # the same values in other places
 
 
 def test_attention_peaked_scores(native):
@@ -496,6 +537,24 @@ def test_linear_slots(native, lens, inplace):
     out = check_linear(native, *x, index=torch.tensor([7, -1, 2]), inplace=inplace, scale=0.7)
     assert bool((out[:3] == 0).all()) and bool((out[-70:] == 0).all())
     check_linear(native, *x, index=torch.tensor([0, 9, 8]), inplace=inplace)
+
+
+@pytest.mark.parametrize("T", [1, 70])
+def test_linear_state_past_32_bits(native, T):
+    """A slot more than 2^31 values into the pool of states."""
+    vh, slots = 32, 4100
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 9 GB of the GPU's memory")
+    q, k, v, a, cu, state, beta = (x.cuda() for x in linear_inputs(8, [T, T], 16, vh, 128, 128))
+    pool = torch.empty((slots, vh, 128, 128), device="cuda")
+    at = torch.tensor([slots - 1, 2], dtype=torch.int32, device="cuda")
+    pool[slots - 1], pool[2] = state[0], state[1]
+    pool[slots - 2] = 5.0
+    got = native.linear_attention(q, k, v, a, cu, pool, beta=beta, state_index=at)
+    ref = native.linear_attention(q, k, v, a, cu, state, beta=beta)
+    assert torch.equal(got, ref)
+    assert torch.equal(pool[slots - 1], state[0]) and torch.equal(pool[2], state[1])
+    assert bool((pool[slots - 2] == 5.0).all())
 
 
 def test_linear_strided(native):

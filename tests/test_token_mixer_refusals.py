@@ -123,6 +123,12 @@ def test_attention_refusals():
     assert call(n=0, q=rows(x=None), table=None, lengths=None, out=None) == _lib.RMOE_OK
 
 
+def test_attention_refuses_a_table_backwards():
+    lib = _lib.load()
+    assert lib.rmoe_paged_attention(ctypes.byref(rows()), ctypes.byref(cache()), FAKE, -4, 4, FAKE, 2, 0, 0.1, FAKE,
+                                    None, FAKE, 1 << 30, None) == _lib.RMOE_EINVAL
+
+
 def test_linear_refusals():
     lib = _lib.load()
     gate = _lib.Gate(FAKE, 4, 1)

@@ -701,8 +701,9 @@ E4M3 = torch.float8_e4m3fn
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
+_current_device = torch._C._cuda_getDevice  # behind tensors that are on a GPU
 _four = ctypes.c_int32 * 4
+_dense = torch.contiguous_format
 
 
 def _one_device(*tensors) -> int:
@@ -831,7 +832,7 @@ def paged_tables(cached: torch.Tensor, added: torch.Tensor, block_table: torch.T
     if rows < 0:
         raise ValueError(f"rows must not be negative (got {rows})")
     ints = torch.empty(2 * rows + 2 * R + 4, dtype=torch.int32, device=device)
-    positions, requests, cu, lengths, counts = ints.split([rows, rows, R + 1, R, 3])
+    positions, requests, cu, lengths, counts = ints.split_with_sizes([rows, rows, R + 1, R, 3])
     slots = torch.empty(rows, dtype=torch.int64, device=device)
     at = ints.data_ptr()
     _call(index, lib.rmoe_paged_tables, cached.data_ptr(), added.data_ptr(), R,
@@ -870,12 +871,11 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
     beyond)."""
     lib = _lib.load()
     index = _one_device(q, k, positions, inv_freq)
-    device = q.device
     q, qr = _heads(q, "q")
     k, kr = _heads(k, "k", q.shape[0], None, q.shape[2])
     spec, positions = _rotary_spec(inv_freq, positions, q.shape[0], sections, woven, adjacent)
-    q_out = torch.empty(q.shape, dtype=BF16, device=device)
-    k_out = torch.empty(k.shape, dtype=BF16, device=device)
+    q_out = torch.empty_like(q, memory_format=_dense)
+    k_out = torch.empty_like(k, memory_format=_dense)
     _call(index, lib.rmoe_rotary, ctypes.byref(spec), positions.data_ptr(), q.shape[0], q.shape[0],
           q.shape[2], ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), k_out.data_ptr())
     return q_out, k_out
@@ -906,7 +906,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     if slots.dtype is not torch.int64 or slots.shape != (N,):
         raise ValueError(f"slots must be int64 [{N}] (got {slots.dtype} {list(slots.shape)})")
     slots = slots.contiguous()
-    q_out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    q_out = torch.empty_like(q, memory_format=_dense)
     _call(index, lib.rmoe_rotary_append, ctypes.byref(spec), positions.data_ptr(), N, N,
           ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), ctypes.byref(vr),
           ctypes.byref(cache), slots.data_ptr())
@@ -939,7 +939,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     P = block_table.shape[1]
     if scale is None:
         scale = D ** -0.5
-    out = torch.empty((R, heads, D), dtype=BF16, device=device)
+    out = torch.empty_like(q, memory_format=_dense)
     lse = torch.empty((R, heads), dtype=torch.float32, device=device) if return_lse else None
     need = lib.rmoe_paged_attention_workspace_bytes(ctypes.byref(cache), heads, R, P, window)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
@@ -1009,7 +1009,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         scale = dk ** -0.5
     if R == 0:
         return torch.zeros((N, vh, dv), dtype=BF16, device=device)
-    out = torch.empty((N, vh, dv), dtype=BF16, device=device)
+    out = torch.empty_like(v, memory_format=_dense)
     need = lib.rmoe_linear_attention_workspace_bytes(N, R, kh, vh, dk, int(gate is not None))
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call(index, lib.rmoe_linear_attention, ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr),

@@ -621,10 +621,20 @@ int64_t attention_keys(int page_size, int width, int window) {
   return window > 0 && window < all ? window : all;
 }
 
-size_t attention_part_bytes(int64_t heads, int splits, int dim, size_t* ml_offset) {
-  const size_t o = (size_t)heads * splits * dim * sizeof(float);
-  if (ml_offset) *ml_offset = o;
-  return splits > 1 ? o + (size_t)heads * splits * sizeof(float2) : 0;
+// Where the parts' maxima and sums, and the requests' lists, lie behind their
+// outputs; the whole without parts is nothing.
+struct PartLayout {
+  size_t ml, list, total;
+};
+
+PartLayout attention_layout(const rmoe::AttentionPlan& plan, int requests, int heads, int dim) {
+  PartLayout l{};
+  if (!plan.parts) return l;
+  const size_t rows = (size_t)plan.all_parts * heads;
+  l.ml = rows * dim * sizeof(float);
+  l.list = l.ml + rows * sizeof(float2);
+  l.total = l.list + (size_t)requests * sizeof(int2);
+  return l;
 }
 
 }  // namespace
@@ -1189,10 +1199,10 @@ size_t rmoe_paged_attention_workspace_bytes(const rmoe_paged_cache* cache, int32
   if (!cache || check_page_size(cache->page_size) || cache->kv_heads < 1 || q_heads < 1 ||
       q_heads % cache->kv_heads || requests < 1 || table_width < 0)
     return 0;
-  const int splits =
+  const rmoe::AttentionPlan plan =
       rmoe::attention_plan(requests, cache->kv_heads, q_heads / cache->kv_heads, cache->dim,
-                           attention_keys(cache->page_size, table_width, window)).splits;
-  return attention_part_bytes((int64_t)requests * q_heads, splits, cache->dim, nullptr);
+                           attention_keys(cache->page_size, table_width, window));
+  return attention_layout(plan, requests, q_heads, cache->dim).total;
 }
 
 int rmoe_paged_attention(const rmoe_rows* q, const rmoe_paged_cache* cache,
@@ -1232,20 +1242,20 @@ int rmoe_paged_attention(const rmoe_rows* q, const rmoe_paged_cache* cache,
   const rmoe::AttentionPlan plan =
       rmoe::attention_plan(requests, a.kv_heads, a.group, a.dim,
                            attention_keys(cache->page_size, table_width, window));
-  a.splits = plan.splits, a.alone = plan.alone;
+  a.parts = plan.parts, a.all_parts = plan.all_parts, a.alone = plan.alone;
   a.out = out, a.lse = lse;
   const int64_t heads = (int64_t)requests * q->heads;
   if (heads * (a.dim / 32) > kMaxGroups ||
-      (int64_t)requests * a.kv_heads * a.head_tiles * a.splits > kMaxGroups)
+      ((int64_t)a.all_parts + 8) * a.kv_heads * a.head_tiles > kMaxGroups)
     return fail(RMOE_EINVAL, "too many requests times heads for one call");
-  size_t ml;
-  const size_t need = attention_part_bytes(heads, a.splits, a.dim, &ml);
-  if (need) {
-    if (!workspace || workspace_bytes < need)
-      return fail(RMOE_EWS, "workspace of %zu bytes needed (got %zu)", need, workspace_bytes);
+  if (a.parts) {
+    const PartLayout l = attention_layout(plan, requests, q->heads, a.dim);
+    if (!workspace || workspace_bytes < l.total)
+      return fail(RMOE_EWS, "workspace of %zu bytes needed (got %zu)", l.total, workspace_bytes);
     if (!aligned(workspace, 16)) return fail(RMOE_EALIGN, "workspace must be 16-byte aligned");
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + ml);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + l.ml);
+    a.list = reinterpret_cast<int2*>(static_cast<char*>(workspace) + l.list);
   }
   const hipError_t e = rmoe::launch_attention(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");

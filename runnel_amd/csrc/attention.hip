@@ -22,8 +22,8 @@
 //     step, 2^-9, of numbers that are averaged; the sum is of the unrounded
 //     ones); everything else is fp32.
 //
-// A request's keys are split over several workgroups and, in each, over its
-// four waves; a second launch joins the workgroups' parts in their order.
+// Requests' keys are split over several workgroups and, in each, over its
+// four waves; a second launch joins a request's parts in their order.
 #include <type_traits>
 
 #include "common.h"
@@ -41,6 +41,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int kAttWaves = 4;  // of a workgroup that shares a request's keys with others
 constexpr int kAttTile = 32;  // keys of a step
 constexpr float kLn2 = 0.69314718056f;
+constexpr int kScanned = 256;  // requests up to which the parts are evened out over all
 
 __device__ __forceinline__ bf16x8 frag(const uint32_t (&w)[4]) {
   union {
@@ -115,31 +116,112 @@ struct Runs {
   static constexpr int second = D - first;
 };
 
-// What the split of a request comes to: its keys [start, end), the tiles of
-// 32 they touch, and how many of them each workgroup takes.
-struct Share {
-  int start, end;   // keys
-  int tile0;        // first tile
-  int tiles;        // of the request
-  int per;          // of a workgroup
-  int parts;        // workgroups with work
+// A request's keys [start, end) and the tiles of 32 they touch.
+struct Keys {
+  int start, end;
+  int tile0, tiles;
 };
 
-__device__ __forceinline__ Share share_of(const AttentionArgs& a, int r) {
-  Share s;
+__device__ __forceinline__ Keys keys_of(const AttentionArgs& a, int r) {
+  Keys s;
   const int64_t most = (int64_t)a.width << a.shift;
   const int len = (int)(a.lengths[r] < most ? a.lengths[r] : most);
   s.end = len > 0 ? len : 0;
   s.start = a.window > 0 && s.end > a.window ? s.end - a.window : 0;
   s.tile0 = s.start / kAttTile;
   s.tiles = s.end > s.start ? (s.end - 1) / kAttTile + 1 - s.tile0 : 0;
-  // no workgroup under a.least tiles while there is another
-  int want = (s.tiles + a.least - 1) / a.least;
-  want = want < a.splits ? want : a.splits;
-  want = want > 0 ? want : 1;
-  s.per = (s.tiles + want - 1) / want;
-  s.parts = s.per ? (s.tiles + s.per - 1) / s.per : 0;
   return s;
+}
+
+// Part `number` of `request`, whose parts are [first, first + as many as it
+// has) of all requests' and take about `per` tiles each.
+struct Part {
+  int request, number, first, per;
+};
+
+__device__ __forceinline__ int ceil_div(int n, int d) { return (int)(((unsigned)n + d - 1) / d); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v) {  // 0 where there is none
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+
+// The sum of the lanes up to this one.
+template <typename T>
+__device__ __forceinline__ T running_sum(T v) {
+  static_assert(sizeof(T) == 4, "one register");
+  auto add = [&](uint32_t u) {
+    T x;
+    __builtin_memcpy(&x, &u, 4);
+    v += x;
+  };
+  auto bits = [&] {
+    uint32_t u;
+    __builtin_memcpy(&u, &v, 4);
+    return u;
+  };
+  add(from_lane<0x111, 0xf>(bits()));  // one lane to the left in a row of 16, then 2, 4, 8
+  add(from_lane<0x112, 0xf>(bits()));
+  add(from_lane<0x114, 0xf>(bits()));
+  add(from_lane<0x118, 0xf>(bits()));
+  add(from_lane<0x142, 0xa>(bits()));  // a row's last lane to the next row, of 32 to the next 32
+  add(from_lane<0x143, 0xc>(bits()));
+  return v;
+}
+
+// Part w of all.  Every wave works it out from the lengths (a load and two
+// running sums across the wave for each 64 requests): the parts of all
+// requests are of about one size, total / a.parts, and there is none without
+// work but the one that a request without keys needs for its zeros.  (With a
+// fixed number of parts for each request, as for more requests than a wave
+// scans, 61 requests of 17 to 16000 keys took 84 us for 72, and 24 for 8 if
+// none had a key: the time of workgroups that find nothing to do.)
+__device__ __forceinline__ Part part_of(const AttentionArgs& a, int w) {
+  if (!a.parts) return {w < a.requests ? w : -1, 0, w, 0x7FFFFFFF};
+  if (a.requests == 1) {
+    const int per = ceil_div(keys_of(a, 0).tiles, a.parts);
+    return {0, w, 0, per > a.least ? per : a.least};
+  }
+  const int lane = threadIdx.x & 63;
+  if (a.requests > kScanned) {  // each request by itself
+    const int each = a.parts / a.requests;
+    const int r = w / each;
+    if (r >= a.requests) return {-1, 0, 0, 0};
+    const int per = ceil_div(keys_of(a, r).tiles, each);
+    return {r, w - r * each, r * each, per > a.least ? per : a.least};
+  }
+  constexpr int N = kScanned / kWave;
+  int n[N];
+  float total = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (kWave * j >= a.requests) break;
+    const int i = lane + kWave * j;
+    n[j] = i < a.requests ? keys_of(a, i).tiles : 0;
+    total += (float)n[j];
+  }
+  total = running_sum(total);
+  total = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(total), kWave - 1));
+  const int even = (int)__builtin_ceilf(total / (float)a.parts);
+  const int per = even > a.least ? even : a.least;
+  int before = 0, r = -1, first = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (kWave * j >= a.requests) break;
+    const int i = lane + kWave * j;
+    int mine = ceil_div(n[j], per);
+    mine = i >= a.requests ? 0 : mine > 0 ? mine : 1;
+    const int upto = running_sum(mine);
+    const int start = before + upto - mine;
+    const uint64_t at = __ballot(start <= w && w < start + mine);
+    if (at) {
+      const int l = __builtin_ctzll(at);
+      r = kWave * j + l;
+      first = __builtin_amdgcn_readlane(start, l);
+    }
+    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return {r, w - first, first, per};
 }
 
 template <int D, bool E4M3, int WAVES>
@@ -157,18 +239,32 @@ void attention_kernel(const AttentionArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  // (split, head tile, key head, request), the request slowest
-  int b = blockIdx.x;
-  const int split = b % a.splits;
-  b /= a.splits;
-  const int ht = b % a.head_tiles;
-  b /= a.head_tiles;
-  const int hk = b % a.kv_heads;
-  const int r = b / a.kv_heads;
-  const Share sh = share_of(a, r);
-  const int t_begin = split * sh.per;
-  const int t_end = t_begin + sh.per < sh.tiles ? t_begin + sh.per : sh.tiles;
-  if (split > 0 && t_begin >= sh.tiles) return;
+  // eight parts side by side, one for each XCD, which takes all heads of its
+  // pages one after the other (heads on XCDs of their own: each XCD goes
+  // through all pages, 8 requests of 100 to 60000 keys 83 us for 53); fewer
+  // parts than that are spread with the heads
+  const int all_heads = a.kv_heads * a.head_tiles;
+  int w, h0;
+  if (a.all_parts >= 8) {
+    const int b = blockIdx.x >> 3;
+    h0 = b % all_heads;
+    w = b / all_heads * 8 + (blockIdx.x & 7);
+  } else {
+    h0 = blockIdx.x % all_heads;
+    w = blockIdx.x / all_heads;
+  }
+  const Part part = part_of(a, w);
+  const int r = __builtin_amdgcn_readfirstlane(part.request);
+  if (r < 0) return;
+  const int ht = h0 % a.head_tiles, hk = h0 / a.head_tiles;
+  const Keys sh = keys_of(a, r);
+  const int want = ceil_div(sh.tiles, part.per);
+  const int per = want > 1 ? ceil_div(sh.tiles, want) : sh.tiles;
+  const int parts = want > 1 ? ceil_div(sh.tiles, per) : 1;
+  if (part.number >= parts) return;
+  if (a.parts && h0 == 0 && part.number == 0 && tid == 0) a.list[r] = make_int2(part.first, parts);
+  const int t_begin = part.number * per;
+  const int t_end = t_begin + per < sh.tiles ? t_begin + per : sh.tiles;
 
   const int left = a.group - ht * 16;
   const int heads = left < 16 ? left : 16;  // of this workgroup
@@ -410,15 +506,15 @@ void attention_kernel(const AttentionArgs a) {
       const int i = tid + q * THREADS;
       if (i >= heads * P) continue;
       const int h = i / P, d = D0 + i - h * P;
-      if (a.splits == 1) {
+      if (parts == 1) {
         const bool some = sum[q] > 0.0f || sum[q] != sum[q];
         a.out[(row + h) * D + d] = (uint16_t)f32_to_bf16(some ? acc[q] / sum[q] * a.v_scale : 0.0f);
         if (a.lse && d == 0)
           a.lse[row + h] = top[q] == -INFINITY ? top[q] : (top[q] + log2f(sum[q])) * kLn2;
       } else {
-        const int64_t part = (row + h) * a.splits + split;
-        a.part_o[part * D + d] = acc[q];
-        if (d == 0) a.part_ml[part] = make_float2(top[q], sum[q]);
+        const int64_t at = (int64_t)w * a.kv_heads * a.group + head0 + h;
+        a.part_o[at * D + d] = acc[q];
+        if (d == 0) a.part_ml[at] = make_float2(top[q], sum[q]);
       }
     }
   };
@@ -439,22 +535,25 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const int64_t row = blockIdx.x / SLICES;  // request and head
   const int slice = blockIdx.x % SLICES;
   const int heads = a.kv_heads * a.group;
-  const Share sh = share_of(a, (int)(row / heads));
+  const int2 list = a.list[row / heads];
+  const int parts = list.y;
+  if (parts == 1) return;  // written in the first launch
+  const int64_t first = (int64_t)list.x * heads + row % heads;
   const int tid = threadIdx.x, c = tid % C, q = tid / C;
   float top = -INFINITY;
-  const float2* ml = a.part_ml + row * a.splits;
-  for (int i = tid & 63; i < sh.parts; i += 64) top = fmaxf(top, ml[i].x);
+  const float2* ml = a.part_ml + first;
+  for (int i = tid & 63; i < parts; i += 64) top = fmaxf(top, ml[(int64_t)i * heads].x);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
   const float base = top == -INFINITY ? 0.0f : top;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
 #pragma unroll 4
-  for (int i = q; i < (q < Q ? sh.parts : 0); i += Q) {
-    const float2 e = ml[i];
+  for (int i = q; i < (q < Q ? parts : 0); i += Q) {
+    const float2 e = ml[(int64_t)i * heads];
     const float f = __builtin_amdgcn_exp2f(e.x - base);
-    const float4 v =
-        reinterpret_cast<const float4*>(a.part_o + (row * a.splits + i) * D + slice * SLICE)[c];
+    const float* part = a.part_o + (first + (int64_t)i * heads) * D + slice * SLICE;
+    const float4 v = reinterpret_cast<const float4*>(part)[c];
     sum += f * e.y;
     acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
   }
@@ -487,7 +586,8 @@ constexpr int kAloneWaves = 8;  // of a workgroup that has a request to itself
 template <int D, bool E4M3>
 hipError_t launch_attention_of(const AttentionArgs& a, hipStream_t s) {
   const int heads = a.group < 16 ? a.group : 16;
-  const unsigned grid = (unsigned)((int64_t)a.requests * a.kv_heads * a.head_tiles * a.splits);
+  const int64_t parts = a.all_parts >= 8 ? (a.all_parts + 7) / 8 * 8 : a.all_parts;
+  const unsigned grid = (unsigned)(parts * a.kv_heads * a.head_tiles);
   auto lds = [&](int waves) {
     return (size_t)(4 * heads * Runs<D>::first + 2 * waves * 16) * sizeof(float);
   };
@@ -498,7 +598,7 @@ hipError_t launch_attention_of(const AttentionArgs& a, hipStream_t s) {
   }
   attention_kernel<D, E4M3, kAttWaves><<<grid, kAttWaves * kWave, lds(kAttWaves), s>>>(a);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
+  if (e != hipSuccess || !a.parts) return e;
   const unsigned rows = (unsigned)(a.requests * a.kv_heads * a.group);
   if (rows <= 256)
     attention_join_kernel<D, 32><<<rows * (D / 32), 256, 0, s>>>(a);
@@ -522,22 +622,32 @@ hipError_t launch_attention_dim(const AttentionArgs& a, hipStream_t s) {
 constexpr int64_t kAloneValues = 512 * 128;
 
 AttentionPlan attention_plan(int requests, int kv_heads, int group, int dim, int64_t keys) {
-  const int64_t base = (int64_t)requests * kv_heads * ((group + 15) / 16);
+  const int64_t heads = (int64_t)kv_heads * ((group + 15) / 16);
+  const int64_t base = requests * heads;
   const int64_t tiles = (keys + kAttTile - 1) / kAttTile;
-  if (base < 256 && tiles > kAttWaves && keys * dim <= kAloneValues) return {1, 1};
-  // a workgroup for every compute unit (131071 keys of 2 heads: 53 us at 128
-  // splits, 62 at 256); more where a request may be long, since the others
-  // may be short (61 requests of 17 to 16000 keys, 8 heads: 119 us at 2
-  // splits, 70 at 8); but no great many that find nothing to do (256 heads'
-  // worth of requests at 64 splits: half of the time)
-  int64_t want = (256 + base - 1) / base;
-  int64_t more = (keys + 2047) / 2048;
-  const int64_t most_groups = (8192 + base - 1) / base;
-  if (more > most_groups) more = most_groups;
-  if (more > want) want = more;
-  const int64_t most = (tiles + kAttWaves - 1) / kAttWaves;
-  want = want < most ? want : most;
-  return {(int)(want < 1 ? 1 : want), 0};
+  const AttentionPlan whole = {0, requests, 0};
+  if (base < 256 && tiles > kAttWaves && keys * dim <= kAloneValues) return {0, requests, 1};
+  // many requests of few keys at most: the second launch would cost more than
+  // uneven ones (64 requests x 8 heads x 2048 keys: 53 us whole, 63 in halves)
+  if (tiles <= kAttWaves || (base >= 256 && keys <= 2048)) return whole;
+  if (requests > kScanned) {
+    const int64_t some = (keys + 2047) / 2048, each = 8192 / base < some ? 8192 / base : some;
+    return each > 1 ? AttentionPlan{(int)(each * requests), (int)(each * requests), 0} : whole;
+  }
+  // Workgroups: of wide heads, whose registers leave room for one or two a
+  // compute unit, one each (4 requests of 1000 to 40000 keys, 2 heads of 256:
+  // 31 us, 40 with 512, 60 with 1024); of others two for a single request
+  // (131071 keys, 8 heads of 128, 8 bits: 57 us, 63 with 1536), and six where
+  // requests differ (61 of 17 to 16000 keys, 8 heads: 72 us, 83 with 512, 75
+  // with 4096).  Where that is less than a part a request, the parts are of
+  // the average request's size (256 of 700 to 4100 keys, 16 heads of 64: 367
+  // us, with larger ones 392).
+  int64_t parts = (dim > 128 ? 256 : requests == 1 ? 512 : 1536) / heads;
+  if (parts < requests) parts = requests;
+  const int64_t most = (tiles + kAttWaves - 1) / kAttWaves * requests;
+  if (parts > most) parts = most;
+  if (parts < 2) return whole;
+  return {(int)parts, (int)(requests == 1 ? parts : parts + requests), 0};
 }
 
 hipError_t launch_attention(const AttentionArgs& in, hipStream_t s) {

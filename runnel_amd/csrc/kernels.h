@@ -265,15 +265,17 @@ struct AttentionArgs {
   const int32_t* lengths;
   int window;                 // 0: all keys
   float scale_log2, v_scale;  // k's scale and log2(e) are in the first
-  int splits, least;          // workgroups of a request, tiles of each at least
+  int parts, all_parts;       // wanted of all requests (0: each whole), there may be
+  int least;                  // tiles of a part at least
   int alone;                  // one workgroup of many waves instead
   uint16_t* out;              // [requests, kv_heads * group, dim]
   float* lse;                 // [requests, heads] or NULL
-  float* part_o;              // [requests, heads, splits, dim] (splits > 1)
-  float2* part_ml;            // [requests, heads, splits]
+  float* part_o;              // [all_parts, heads, dim] (with parts)
+  float2* part_ml;            // [all_parts, heads]
+  int2* list;                 // [requests]: its first part, how many
 };
 struct AttentionPlan {
-  int splits, alone;
+  int parts, all_parts, alone;
 };
 AttentionPlan attention_plan(int requests, int kv_heads, int group, int dim, int64_t keys);
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t s);

@@ -353,6 +353,32 @@ def test_attention_long(native):
     check_attention(native, *attention_inputs(2, [20011], 2, 1, 64, 32, 8), ks=0.5, vs=0.5)
 
 
+@pytest.mark.parametrize("R", [2, 3, 64, 65, 200, 256, 257])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_attention_ragged(native, R, bits):
+    """A long request or two among short and empty ones, whose parts lie
+    anywhere among all requests': in one, two and four runs of 64 requests,
+    and more requests than are looked through."""
+    lens = [(0, 1, 33, 5, 190, 0, 64)[i * 5 % 7] for i in range(R)]
+    lens[R // 2], lens[-1] = 2500, 1300
+    if R > 70:
+        lens[63], lens[64] = 700, 0
+    check_attention(native, *attention_inputs(R, lens, 3, 1, 64, 32, bits))
+    # all without a key but one, none at all
+    q, kc, vc, table, lengths = attention_inputs(R, lens, 3, 1, 64, 32, bits)
+    for keep in (R // 2, None):
+        some = torch.tensor([n if i == keep else 0 for i, n in enumerate(lens)], dtype=torch.int32)
+        check_attention(native, q, kc, vc, table, some)
+
+
+@pytest.mark.parametrize("hq,hk", [(40, 2), (6, 6)])
+def test_attention_ragged_heads(native, hq, hk):
+    """Several heads of keys, and more than a tile of query heads to one."""
+    lens = [3, 2100, 0, 40, 900, 1, 2, 65, 350]
+    check_attention(native, *attention_inputs(5, lens, hq, hk, 64, 16, 16))
+    check_attention(native, *attention_inputs(5, lens, hq, hk, 64, 16, 16), window=777)
+
+
 def test_attention_bad_pages(native):
     """Pages outside the cache, a length past the table and one below 0."""
     q, kc, vc, table, lengths = attention_inputs(5, [100, 100, 64, 40], 4, 2, 64, 8, 16)

@@ -4,7 +4,8 @@ Drop-in surfaces:
   fuse_routed_gate_up(model) -> int, FusedQuantizedSwitchGLU
       (the reference's src/runnel/mlx.py:8-95)
   SparseMoeBlock   the mlx-lm block that calls the packed module
-  native.*         torch-facing wrappers of the C ABI in include/rmoe.h
+  native.*         torch-facing wrappers of the C ABI in include/rmoe.h, the
+                   token mixer's operators for serving among them
 The compute runs in runnel_amd/librmoe.so (hand-written HIP for gfx950).
 """
 

@@ -706,24 +706,23 @@ _four = ctypes.c_int32 * 4
 _dense = torch.contiguous_format
 
 
-def _one_device(*tensors) -> int:
-    """The index of the GPU that all of the tensors are on; refuses tensors
-    that want a gradient (the operators below have no backward pass)."""
-    index = None
-    grad = torch.is_grad_enabled()
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("runnel_amd kernels take GPU tensors")
-        i = t.get_device()
-        if index is None:
-            index = i
-        elif i != index:
+def _one_device(first, *others) -> int:
+    """The index of the GPU that all of the tensors (or None) are on; refuses
+    tensors that want a gradient (the operators below have no backward pass)."""
+    index = first.get_device()  # -1: not on a GPU
+    for t in others:
+        if t is not None and t.get_device() != index:
+            i = t.get_device()
+            if index < 0 or i < 0:
+                raise ValueError("runnel_amd kernels take GPU tensors")
             raise ValueError(f"tensors are on cuda:{index} and cuda:{i}")
-        if grad and t.requires_grad:
-            raise ValueError("this operator has no backward pass: call it under torch.no_grad() "
-                             "or on detached tensors")
+    if index < 0:
+        raise ValueError("runnel_amd kernels take GPU tensors")
+    if torch.is_grad_enabled():
+        for t in (first, *others):
+            if t is not None and t.requires_grad:
+                raise ValueError("this operator has no backward pass: call it under "
+                                 "torch.no_grad() or on detached tensors")
     return index
 
 

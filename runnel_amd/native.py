@@ -700,8 +700,9 @@ def dequantize(weight, scales, biases, bits: int, group_size: int = 64,
 E4M3 = torch.float8_e4m3fn
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice  # behind tensors that are on a GPU
+# (absent from a torch that was built without GPUs)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 _four = ctypes.c_int32 * 4
 _dense = torch.contiguous_format
 

@@ -695,104 +695,23 @@ def dequantize(weight, scales, biases, bits: int, group_size: int = 64,
 # rotary positions written through to it, attention of one new token over
 # it, and linear attention over a recurrent state.  None of these keeps
 # anything between calls: their scratch comes from torch's allocator for each
-# call, so calls on several streams and captured graphs share nothing.
+# call, so calls on several streams and captured graphs share nothing.  Checks
+# and allocations are compiled (csrc/mixer_py.cpp, runnel_amd/_mixer.so).
 
-E4M3 = torch.float8_e4m3fn
-
-
-# (absent from a torch that was built without GPUs)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
-_four = ctypes.c_int32 * 4
-_dense = torch.contiguous_format
+_mixer = None
 
 
-def _one_device(first, *others) -> int:
-    """The index of the GPU that all of the tensors (or None) are on; refuses
-    tensors that want a gradient (the operators below have no backward pass)."""
-    index = first.get_device()  # -1: not on a GPU
-    for t in others:
-        if t is not None and t.get_device() != index:
-            i = t.get_device()
-            if index < 0 or i < 0:
-                raise ValueError("runnel_amd kernels take GPU tensors")
-            raise ValueError(f"tensors are on cuda:{index} and cuda:{i}")
-    if index < 0:
-        raise ValueError("runnel_amd kernels take GPU tensors")
-    if torch.is_grad_enabled():
-        for t in (first, *others):
-            if t is not None and t.requires_grad:
-                raise ValueError("this operator has no backward pass: call it under "
-                                 "torch.no_grad() or on detached tensors")
-    return index
-
-
-def _call(index: int, function, *args) -> None:
-    """`function` of the library, on GPU `index` and torch's current stream there."""
-    if index == _current_device():
-        rc = function(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = function(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc)
-
-
-def _int32(t: torch.Tensor, name: str, shape) -> torch.Tensor:
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
-    if t.dtype is torch.int32 and t.is_contiguous():
-        return t
-    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-        raise ValueError(f"{name} must be int32 (got {t.dtype})")
-    return t.to(torch.int32).contiguous()
-
-
-def _heads(t: torch.Tensor, name: str, rows: int | None = None, heads: int | None = None,
-           dim: int | None = None):
-    """A bf16 [rows, heads, dim] tensor and its rmoe_rows: as it lies where the
-    kernels can read it so (a slice of a packed projection), else copied."""
-    shape = t.shape
-    if t.dtype is not BF16 or len(shape) != 3:
-        raise ValueError(f"{name} must be a bfloat16 [rows, heads, dim] tensor "
-                         f"(got {t.dtype} {list(shape)})")
-    if (rows is not None and shape[0] != rows or heads is not None and shape[1] != heads
-            or dim is not None and shape[2] != dim):
-        want = [n if m is None else m for n, m in zip(shape, (rows, heads, dim))]
-        raise ValueError(f"{name} must be {want} (got {list(shape)})")
-    row, head, one = t.stride()
-    address = t.data_ptr()
-    if one != 1 or row % 8 or head % 8 or address % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        row, head, one = t.stride()
-        address = t.data_ptr()
-        if row % 8 or head % 8:
-            raise ValueError(f"{name}'s dim must be a multiple of 8 (got {shape[2]})")
-    return t, _lib.Rows(address, row, head, shape[1])
-
-
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: float,
-           v_scale: float) -> _lib.PagedCache:
-    eight = k_cache.dtype is E4M3
-    if not eight and k_cache.dtype is not BF16:
-        raise ValueError(f"the cache must be bfloat16 or float8_e4m3fn (got {k_cache.dtype})")
-    shape = k_cache.shape
-    if len(shape) != 4:
-        raise ValueError("the cache must be [pages, kv heads, page size, dim] "
-                         f"(got {list(shape)})")
-    if v_cache.dtype is not k_cache.dtype or v_cache.shape != shape:
-        raise ValueError("k_cache and v_cache must have one type and shape")
-    # (a dimension of one has no stride)
-    ks = [0 if n == 1 else st for n, st in zip(shape, k_cache.stride())]
-    if v_cache.stride() != k_cache.stride() and ks != [
-            0 if n == 1 else st for n, st in zip(shape, v_cache.stride())]:
-        raise ValueError("k_cache and v_cache must lie in memory alike")
-    if ks[3] != 1:
-        raise ValueError("the cache's last dimension must be contiguous")
-    if not eight and (k_scale != 1.0 or v_scale != 1.0):
-        raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], shape[0],
-                           shape[2], shape[1], shape[3], 8 if eight else 16, k_scale, v_scale)
+def _binding():
+    global _mixer
+    if _mixer is None:
+        _lib.load()
+        try:
+            from . import _mixer as built
+        except ImportError as e:
+            raise RuntimeError("runnel_amd/_mixer.so is missing or was built for another torch: "
+                               "build it with `make -C runnel_amd/csrc`") from e
+        _mixer = built
+    return _mixer
 
 
 @dataclass
@@ -819,44 +738,8 @@ def paged_tables(cached: torch.Tensor, added: torch.Tensor, block_table: torch.T
     the caller takes ``counts[1]`` pages off the list's front).  `rows` is the
     row count of the step's batch: tokens of all requests one after the
     other, rows behind the last one marked -1."""
-    lib = _lib.load()
-    index = _one_device(cached, added, block_table, free_pages)
-    device = block_table.device
-    if block_table.dtype != torch.int32 or block_table.dim() != 2:
-        raise ValueError("block_table must be int32 [requests, pages]")
-    R, P = block_table.shape
-    if P > 1 and block_table.stride(1) != 1:
-        raise ValueError("block_table's rows must be contiguous (it is updated in place)")
-    cached, added = _int32(cached, "cached", (R,)), _int32(added, "added", (R,))
-    free_pages = _int32(free_pages, "free_pages", (free_pages.numel(),))
-    if rows < 0:
-        raise ValueError(f"rows must not be negative (got {rows})")
-    ints = torch.empty(2 * rows + 2 * R + 4, dtype=torch.int32, device=device)
-    positions, requests, cu, lengths, counts = ints.split_with_sizes([rows, rows, R + 1, R, 3])
-    slots = torch.empty(rows, dtype=torch.int64, device=device)
-    at = ints.data_ptr()
-    _call(index, lib.rmoe_paged_tables, cached.data_ptr(), added.data_ptr(), R,
-          block_table.data_ptr(), max(block_table.stride(0), P) if R == 1 else block_table.stride(0),
-          P, free_pages.data_ptr(), free_pages.numel(), page_size, rows, slots.data_ptr(), at,
-          at + 4 * rows, at + 8 * rows, at + 8 * rows + 4 * (R + 1), at + 8 * rows + 4 * (2 * R + 1))
-    return PagedTables(slots, positions, requests, cu, lengths, counts)
-
-
-def _rotary_spec(inv_freq, positions, rows: int, sections, woven: bool, adjacent: bool):
-    """(rmoe_rotary_spec, positions int32 [axes, rows], its axis stride)."""
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-        raise ValueError("inv_freq must be a contiguous float32 vector")
-    half = inv_freq.numel()
-    if sections is None:
-        sections = (half,)
-    axes = len(sections)
-    if not 1 <= axes <= 4:
-        raise ValueError(f"sections must name 1 to 4 axes (got {axes})")
-    positions = _int32(positions, "positions",
-                       (rows,) if axes == 1 and positions.dim() == 1 else (axes, rows))
-    spec = _lib.RotarySpec(inv_freq.data_ptr(), half, axes, _four(*sections), 1 if woven else 0,
-                           1 if adjacent else 0)
-    return spec, positions
+    return PagedTables(*_binding().paged_tables(cached, added, block_table, free_pages, page_size,
+                                                rows))
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -869,16 +752,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: 
     pairs that sum to len(inv_freq): the axes one section after the other, or
     in turn when `woven` (axis i mod A until its section is used up, axis 0
     beyond)."""
-    lib = _lib.load()
-    index = _one_device(q, k, positions, inv_freq)
-    q, qr = _heads(q, "q")
-    k, kr = _heads(k, "k", q.shape[0], None, q.shape[2])
-    spec, positions = _rotary_spec(inv_freq, positions, q.shape[0], sections, woven, adjacent)
-    q_out = torch.empty_like(q, memory_format=_dense)
-    k_out = torch.empty_like(k, memory_format=_dense)
-    _call(index, lib.rmoe_rotary, ctypes.byref(spec), positions.data_ptr(), q.shape[0], q.shape[0],
-          q.shape[2], ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), k_out.data_ptr())
-    return q_out, k_out
+    return _binding().rotary(q, k, positions, inv_freq, sections, woven, adjacent)
 
 
 def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -891,26 +765,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     strides with contiguous last dimension) at slots int64 [N] (page * page
     size + place, as ``paged_tables`` gives them; -1: nowhere) -> the turned q.
     8-bit caches hold e4m3(x / scale), saturating.  Slots of one call differ."""
-    lib = _lib.load()
-    index = _one_device(q, k, v, positions, inv_freq, k_cache, v_cache, slots)
-    cache = _cache(k_cache, v_cache, k_scale, v_scale)
-    if 0 in k_cache.stride():
-        raise ValueError("an expanded cache cannot be written")
-    if cache.k == cache.v:
-        raise ValueError("k_cache and v_cache must be two")
-    q, qr = _heads(q, "q", None, None, cache.dim)
-    N = q.shape[0]
-    k, kr = _heads(k, "k", N, cache.kv_heads, cache.dim)
-    v, vr = _heads(v, "v", N, cache.kv_heads, cache.dim)
-    spec, positions = _rotary_spec(inv_freq, positions, N, sections, woven, adjacent)
-    if slots.dtype is not torch.int64 or slots.shape != (N,):
-        raise ValueError(f"slots must be int64 [{N}] (got {slots.dtype} {list(slots.shape)})")
-    slots = slots.contiguous()
-    q_out = torch.empty_like(q, memory_format=_dense)
-    _call(index, lib.rmoe_rotary_append, ctypes.byref(spec), positions.data_ptr(), N, N,
-          ctypes.byref(qr), q_out.data_ptr(), ctypes.byref(kr), ctypes.byref(vr),
-          ctypes.byref(cache), slots.data_ptr())
-    return q_out
+    return _binding().rotary_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, sections,
+                                    woven, adjacent, k_scale, v_scale)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -925,35 +781,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     order (Hq a multiple of Hk).  Keys of a page outside the cache (-1) do not
     count.  A request without keys gets zeros.  With return_lse also float32
     [R, Hq], the logarithm of the sum of the exponentials (-inf: no keys)."""
-    lib = _lib.load()
-    index = _one_device(q, k_cache, v_cache, block_table, lengths)
-    device = q.device
-    cache = _cache(k_cache, v_cache, k_scale, v_scale)
-    q, qr = _heads(q, "q", None, None, cache.dim)
-    R, heads, D = q.shape
-    if block_table.dim() != 2 or block_table.shape[0] != R:
-        raise ValueError(f"block_table must be [{R}, pages] (got {list(block_table.shape)})")
-    if block_table.dtype is not torch.int32 or block_table.stride(1) != 1:
-        block_table = _int32(block_table, "block_table", block_table.shape)
-    lengths = _int32(lengths, "lengths", (R,))
-    P = block_table.shape[1]
-    if scale is None:
-        scale = D ** -0.5
-    out = torch.empty_like(q, memory_format=_dense)
-    lse = torch.empty((R, heads), dtype=torch.float32, device=device) if return_lse else None
-    need = lib.rmoe_paged_attention_workspace_bytes(ctypes.byref(cache), heads, R, P, window)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _call(index, lib.rmoe_paged_attention, ctypes.byref(qr), ctypes.byref(cache),
-          block_table.data_ptr(), block_table.stride(0), P, lengths.data_ptr(), R, window, scale,
-          out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need)
-    return (out, lse) if return_lse else out
-
-
-def _gate_rows(t: torch.Tensor, name: str, rows: int, heads: int) -> _lib.Gate:
-    if t.dtype is not torch.float32 or t.shape != (rows, heads):
-        raise ValueError(f"{name} must be float32 [{rows}, {heads}] "
-                         f"(got {t.dtype} {list(t.shape)})")
-    return _lib.Gate(t.data_ptr(), *t.stride())
+    return _binding().paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window,
+                                      k_scale, v_scale, return_lse)
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -976,47 +805,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     of state_out (default: state itself), of which no other slot is touched.
     Calls of few tokens per sequence run token by token, others in chunks;
     both hold the state in float32."""
-    lib = _lib.load()
-    index = _one_device(q, k, v, log_decay, cu_seqlens, state, beta, state_index, state_out)
-    device = q.device
-    q, qr = _heads(q, "q")
-    N, kh, dk = q.shape
-    k, kr = _heads(k, "k", N, kh, dk)
-    v, vr = _heads(v, "v", N)
-    vh, dv = v.shape[1:]
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
-        raise ValueError("cu_seqlens must be [sequences + 1]")
-    R = cu_seqlens.numel() - 1
-    cu_seqlens = _int32(cu_seqlens, "cu_seqlens", (R + 1,))
-    decay = _gate_rows(log_decay, "log_decay", N, vh)
-    gate = None if beta is None else _gate_rows(beta, "beta", N, vh)
-    slots = state.shape[0] if state.dim() else 0
-    want = (slots, vh, dk, dv)
-    if state_out is None:
-        state_out = state
-    for t, name in ((state, "state"), (state_out, "state_out")):
-        if t.dtype is not torch.float32 or t.shape != want or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 {list(want)} "
-                             f"(got {t.dtype} {list(t.shape)})")
-    at, to = state.data_ptr(), state_out.data_ptr()
-    if at != to and abs(at - to) < 4 * state.numel():
-        raise ValueError("state_out must be state or lie apart from it")
-    if state_index is not None:
-        state_index = _int32(state_index, "state_index", (R,))
-    elif slots < R:
-        raise ValueError(f"state has {slots} slots for {R} sequences")
-    if scale is None:
-        scale = dk ** -0.5
-    if R == 0:
-        return torch.zeros((N, vh, dv), dtype=BF16, device=device)
-    out = torch.empty_like(v, memory_format=_dense)
-    need = lib.rmoe_linear_attention_workspace_bytes(N, R, kh, vh, dk, int(gate is not None))
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _call(index, lib.rmoe_linear_attention, ctypes.byref(qr), ctypes.byref(kr), ctypes.byref(vr),
-          ctypes.byref(decay), None if gate is None else ctypes.byref(gate), cu_seqlens.data_ptr(),
-          N, R, dk, dv, scale, at, to, _lib.ptr(state_index), slots, out.data_ptr(), 1,
-          _lib.ptr(ws), need)
-    return out
+    return _binding().linear_attention(q, k, v, log_decay, cu_seqlens, state, beta, state_index,
+                                       scale, state_out)
 
 
 def stream_read(buf: torch.Tensor, blocks: int, partials: torch.Tensor | None = None):

@@ -38,6 +38,83 @@ def close(got, ref, tol, name=""):
                            f"{(got - ref).abs()[bad].max().item():.3g}")
 
 
+# ---------------------------------------------------------------- refusals
+
+
+def test_wrapper_checks(native):
+    """The checks that stand between a tensor and its address."""
+    def z(*shape, dtype=BF16):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+    c, q, table, lens = z(4, 2, 16, 64), z(1, 2, 64), z(1, 3, dtype=torch.int32), z(1, dtype=torch.int32)
+
+    def attend(k=c, v=c, q=q, table=table, lens=lens, **kw):
+        return native.paged_attention(q, k, v, table, lens, **kw)
+
+    turned = z(4, 2, 64, 16).transpose(2, 3)
+    for why, kw in (("one type and shape", dict(v=c[:3])), ("one type and shape", dict(v=c.to(E4M3))),
+                    ("lie in memory alike", dict(v=z(4, 16, 2, 64).transpose(1, 2))),
+                    ("contiguous", dict(k=turned, v=turned)), ("belong to float8", dict(k_scale=0.5)),
+                    ("must be bfloat16 or float8", dict(k=c.half(), v=c.half())),
+                    ("cache must be", dict(k=c[0], v=c[0])),
+                    ("q must be", dict(q=z(1, 2, 96))), ("bfloat16", dict(q=z(1, 2, 64, dtype=torch.float32))),
+                    ("block_table must be", dict(table=table[0])), ("block_table must be", dict(table=table[:0])),
+                    ("block_table must be int32", dict(table=table.float())),
+                    ("lengths must be", dict(lens=z(2, dtype=torch.int32))),
+                    ("window", dict(window=-1)), ("window is out of range", dict(window=1 << 33)),
+                    ("multiple of the 2 key heads", dict(q=z(1, 3, 64))),
+                    ("GPU tensors", dict(q=q.cpu())), ("GPU tensors", dict(lens=lens.cpu())),
+                    ("no backward pass", dict(q=q.clone().requires_grad_()))):
+        with pytest.raises(ValueError, match=why):
+            attend(**kw)
+    with torch.no_grad():
+        attend(q=q.clone().requires_grad_())
+    with pytest.raises(TypeError):
+        attend(window=None)
+    # a dimension of one: its stride says nothing
+    one = z(1, 2, 16, 64).as_strided((1, 2, 16, 64), (7, 1024, 64, 1))
+    assert attend(k=c[:1], v=one).shape == (1, 2, 64)
+
+    inv, pos, x = z(32, dtype=torch.float32), z(2, dtype=torch.int32), z(2, 3, 64)
+    for why, args in (("multiple of 8", (z(2, 3, 60), x, pos, inv)), ("k must be", (x, z(3, 3, 64), pos, inv)),
+                      ("k must be", (x, z(2, 3, 96), pos, inv)),
+                      ("1 to 4 axes", (x, x, z(5, 2, dtype=torch.int32), inv, (8, 8, 8, 4, 4))),
+                      ("positions must be", (x, x, pos, inv, (16, 16))),
+                      ("int32", (x, x, pos.float(), inv)), ("float32", (x, x, pos, inv.double())),
+                      ("contiguous float32", (x, x, pos, z(64, dtype=torch.float32)[::2])),
+                      ("sum to half", (x, x, z(2, 2, dtype=torch.int32), inv, (16, 15)))):
+        with pytest.raises(ValueError, match=why):
+            native.rotary(*args)
+    with pytest.raises(TypeError):
+        native.rotary(x, x, z(2, 2, dtype=torch.int32), inv, (16, "16"))
+
+    flat = z(3 * 64 * 64 + 64, dtype=torch.float32)
+    g, cu, st = z(2, 3, dtype=torch.float32), torch.tensor([0, 2], device="cuda"), z(1, 3, 64, 64, dtype=torch.float32)
+
+    def linear(q=x, k=x, v=x, g=g, cu=cu, st=st, **kw):
+        return native.linear_attention(q, k, v, g, cu, st, **kw)
+
+    for why, kw in (("log_decay must be float32", dict(g=g.to(BF16))), ("log_decay must be", dict(g=g[:1])),
+                    ("beta must be", dict(beta=g[:, :2])), ("cu_seqlens must be", dict(cu=cu[:0])),
+                    ("state must be contiguous", dict(st=st.transpose(2, 3))),
+                    ("state_out must be contiguous", dict(state_out=st[:, :2])),
+                    ("lie apart", dict(st=flat[:-64].view(1, 3, 64, 64), state_out=flat[64:].view(1, 3, 64, 64))),
+                    ("slots for 2 sequences", dict(cu=torch.tensor([0, 1, 2], device="cuda"))),
+                    ("state_index must be", dict(state_index=z(2, dtype=torch.int32)))):
+        with pytest.raises(ValueError, match=why):
+            linear(**kw)
+    assert native.linear_attention(x, x, x, g[:1].expand(2, 3), cu, st).shape == (2, 3, 64)
+
+    i = z(2, dtype=torch.int32)
+    for why, args in (("block_table must be int32", (i, i, z(2, 4, dtype=torch.int64), i, 16, 2)),
+                      ("contiguous", (i, i, z(4, 2, dtype=torch.int32).t(), i, 16, 2)),
+                      ("cached must be", (i[:1], i, z(2, 4, dtype=torch.int32), i, 16, 2)),
+                      ("rows must not be negative", (i, i, z(2, 4, dtype=torch.int32), i, 16, -1)),
+                      ("page_size", (i, i, z(2, 4, dtype=torch.int32), i, 12, 2))):
+        with pytest.raises(ValueError, match=why):
+            native.paged_tables(*args)
+
+
 # ---------------------------------------------------------------- the tables
 
 

@@ -171,42 +171,26 @@ def test_wrappers_take_gpu_tensors():
             call()
 
 
-def test_wrapper_checks():
-    """The shape checks that stand between a tensor and its address."""
-    c = torch.zeros(4, 2, 16, 64, dtype=BF16)
-    with pytest.raises(ValueError, match="one type and shape"):
-        native._cache(c, c[:3], 1.0, 1.0)
-    with pytest.raises(ValueError, match="lie in memory alike"):
-        native._cache(c, torch.zeros(4, 16, 2, 64, dtype=BF16).transpose(1, 2), 1.0, 1.0)
-    with pytest.raises(ValueError, match="contiguous"):
-        t = torch.zeros(4, 2, 64, 16, dtype=BF16).transpose(2, 3)
-        native._cache(t, t, 1.0, 1.0)
-    with pytest.raises(ValueError, match="belong to float8"):
-        native._cache(c, c, 0.5, 1.0)
-    with pytest.raises(ValueError, match="must be bfloat16 or float8"):
-        native._cache(c.half(), c.half(), 1.0, 1.0)
-    # a dimension of one: its stride says nothing
-    one = native._cache(c[:1], torch.zeros(1, 2, 16, 64, dtype=BF16).as_strided((1, 2, 16, 64), (7, 1024, 64, 1)),
-                        1.0, 1.0)
-    assert one.page_stride == 0 and one.bits == 16 and one.kv_heads == 2
-    with pytest.raises(ValueError, match=r"must be \[2, 4, 64\]"):
-        native._heads(torch.zeros(2, 3, 64, dtype=BF16), "q", 2, 4, 64)
-    with pytest.raises(ValueError, match="bfloat16"):
-        native._heads(torch.zeros(2, 3, 64), "q")
-    with pytest.raises(ValueError, match="multiple of 8"):
-        native._heads(torch.zeros(2, 3, 60, dtype=BF16), "q")
-    inv = torch.zeros(32)
-    with pytest.raises(ValueError, match="1 to 4 axes"):
-        native._rotary_spec(inv, torch.zeros(5, 2, dtype=torch.int32), 2, (8, 8, 8, 4, 4), False, False)
-    with pytest.raises(ValueError, match="positions must be"):
-        native._rotary_spec(inv, torch.zeros(2, dtype=torch.int32), 2, (16, 16), False, False)
-    with pytest.raises(ValueError, match="int32"):
-        native._rotary_spec(inv, torch.zeros(2), 2, None, False, False)
-    with pytest.raises(ValueError, match="float32"):
-        native._rotary_spec(inv.double(), torch.zeros(2, dtype=torch.int32), 2, None, False, False)
-    with pytest.raises(ValueError, match="log_decay must be float32"):
-        native._gate_rows(torch.zeros(3, 2, dtype=BF16), "log_decay", 3, 2)
-    assert native._gate_rows(torch.zeros(1, 2).expand(9, 2), "g", 9, 2).row_stride == 0
+def test_wrappers_take_tensors():
+    x = torch.zeros(2, 4, 64, dtype=BF16)
+    with pytest.raises(TypeError, match="k must be a tensor"):
+        native.rotary(x, None, x, x)
+    with pytest.raises(TypeError):
+        native.paged_tables(x, x, x, x, 16.5, 2)
+    with pytest.raises(ValueError, match="page_size is out of range"):
+        native.paged_tables(x, x, x, x, 1 << 40, 2)
+
+
+def test_a_binding_that_was_not_built(monkeypatch):
+    import sys
+
+    import runnel_amd
+    native._binding()
+    monkeypatch.setattr(native, "_mixer", None)
+    monkeypatch.delattr(runnel_amd, "_mixer")
+    monkeypatch.setitem(sys.modules, "runnel_amd._mixer", None)
+    with pytest.raises(RuntimeError, match="_mixer.so is missing"):
+        native._binding()
 
 
 def test_oracle_tables():

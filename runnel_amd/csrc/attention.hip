@@ -616,8 +616,8 @@ hipError_t launch_attention_dim(const AttentionArgs& a, hipStream_t s) {
 
 // Up to this many values of K a request that would be split is left whole to
 // one workgroup of eight waves, without a second launch (one request, 2 key
-// heads of 128 dims: 130 keys 8.6 us against 9.7, 500 keys 10.9 against 10.6,
-// and 4 us less on the host; 1000 keys 15.5 against 10.7: one compute unit
+// heads of 128 dims: 130 keys 8.6 us against 9.7, 500 keys 10.9 against 10.6
+// and a launch less on the host; 1000 keys 15.5 against 10.7: one compute unit
 // reads 60 GB/s).
 constexpr int64_t kAloneValues = 512 * 128;
 

@@ -56,6 +56,12 @@ float real(PyObject* o) {
   return (float)v;
 }
 
+bool flag(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v != 0;
+}
+
 // ------------------------------------------------------------------- checks
 
 // The index of the GPU that all of the tensors (or undefined ones) are on;
@@ -70,6 +76,9 @@ int one_device(const std::array<const Tensor*, N>& all) {
     const int i = t->get_device();
     TORCH_CHECK_VALUE(index < 0 || i == index, "tensors are on cuda:", index, " and cuda:", i);
     index = i;
+    // (fake tensors and the like: there may be no memory behind them)
+    TORCH_CHECK_VALUE(!t->key_set().has(c10::DispatchKey::Python),
+                      "tensors whose operations dispatch to Python are not taken");
     TORCH_CHECK_VALUE(!grad || !t->requires_grad(),
                       "this operator has no backward pass: call it under torch.no_grad() or on "
                       "detached tensors");
@@ -203,16 +212,21 @@ void raise_status(int rc) {
   throw python_error();  // check() has raised
 }
 
-// call(stream) on GPU `index` and torch's current stream there.
+struct WithoutGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+
+// call(stream) on GPU `index` and torch's current stream there; other Python
+// threads run meanwhile.
 template <typename F>
 void on_stream(int index, F call) {
   int rc;
   {
-    c10::DeviceGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)index));
+    const c10::DeviceGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)index));
     void* stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)index).stream();
-    Py_BEGIN_ALLOW_THREADS;
+    const WithoutGil without;
     rc = call(stream);
-    Py_END_ALLOW_THREADS;
   }
   if (rc) raise_status(rc);
 }
@@ -273,8 +287,7 @@ PyObject* rotary(PyObject* const* o) {
   const Tensor &positions = tensor(o[2], "positions"), &inv_freq = tensor(o[3], "inv_freq");
   const int index = one_device<4>({&q0, &k0, &positions, &inv_freq});
   const Heads q = heads(q0, "q"), k = heads(k0, "k", q.n, -1, q.dim);
-  const Rotary r = rotary_of(inv_freq, positions, q.n, o[4], PyObject_IsTrue(o[5]) == 1,
-                             PyObject_IsTrue(o[6]) == 1);
+  const Rotary r = rotary_of(inv_freq, positions, q.n, o[4], flag(o[5]), flag(o[6]));
   const Tensor q_out = like(q), k_out = like(k);
   const int32_t n = small(q.n, "the row count"), dim = small(q.dim, "q's dim");
   on_stream(index, [&](void* stream) {
@@ -301,8 +314,7 @@ PyObject* rotary_append(PyObject* const* o) {
   const Heads q = heads(q0, "q", -1, -1, cache.dim);
   const Heads k = heads(k0, "k", q.n, cache.kv_heads, cache.dim);
   const Heads v = heads(v0, "v", q.n, cache.kv_heads, cache.dim);
-  const Rotary r = rotary_of(inv_freq, positions, q.n, o[8], PyObject_IsTrue(o[9]) == 1,
-                             PyObject_IsTrue(o[10]) == 1);
+  const Rotary r = rotary_of(inv_freq, positions, q.n, o[8], flag(o[9]), flag(o[10]));
   TORCH_CHECK_VALUE(slots0.scalar_type() == at::kLong && is(slots0, {q.n}), "slots must be int64 [",
                     q.n, "] (got ", slots0.scalar_type(), " ", slots0.sizes(), ")");
   const Tensor slots = slots0.contiguous(), q_out = like(q);
@@ -332,7 +344,7 @@ PyObject* paged_attention(PyObject* const* o) {
   const float scale = o[5] == Py_None ? (float)(1.0 / std::sqrt((double)q.dim)) : real(o[5]);
   const int32_t window = integer(o[6], "window"), R = small(q.n, "the request count");
   const int32_t width = small(table.size(1), "the table's width");
-  const bool with_lse = PyObject_IsTrue(o[9]) == 1;
+  const bool with_lse = flag(o[9]);
   const Tensor out = like(q);
   const Tensor lse =
       with_lse ? at::empty({q.n, q.rows.heads}, out.options().dtype(at::kFloat)) : Tensor();

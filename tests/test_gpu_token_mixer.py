@@ -41,6 +41,24 @@ def close(got, ref, tol, name=""):
 # ---------------------------------------------------------------- refusals
 
 
+def test_no_rows(native):
+    """Calls of no row at all, of no request and of no sequence."""
+    def z(*shape, dtype=BF16):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+    x, i, c, inv = z(0, 2, 64), z(0, dtype=torch.int32), z(3, 2, 16, 64), z(32, dtype=torch.float32)
+    assert [t.shape for t in native.rotary(x, x, i, inv)] == [(0, 2, 64)] * 2
+    assert native.rotary_append(x, x, x, i, inv, c, c.clone(), i.long()).shape == (0, 2, 64)
+    out, lse = native.paged_attention(x, c, c, z(0, 9, dtype=torch.int32), i, return_lse=True)
+    assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
+    g, st = z(0, 2, dtype=torch.float32), torch.ones(2, 2, 64, 64, device="cuda")
+    for cu in ([0], [0, 0, 0]):
+        out = native.linear_attention(x, x, x, g, torch.tensor(cu, device="cuda"), st, beta=g)
+        assert out.shape == (0, 2, 64) and bool((st == 1).all())
+    t = native.paged_tables(z(2, dtype=torch.int32), z(2, dtype=torch.int32), z(2, 3, dtype=torch.int32), i, 16, 0)
+    assert t.slots.numel() == 0 and t.counts.tolist() == [0, 0, 0]
+
+
 def test_wrapper_checks(native):
     """The checks that stand between a tensor and its address."""
     def z(*shape, dtype=BF16):
@@ -71,6 +89,11 @@ def test_wrapper_checks(native):
         attend(q=q.clone().requires_grad_())
     with pytest.raises(TypeError):
         attend(window=None)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        attend(return_lse=z(2))
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode() as fake, pytest.raises(ValueError, match="dispatch to Python"):
+        attend(lens=fake.from_tensor(lens))  # has no memory
     # a dimension of one: its stride says nothing
     one = z(1, 2, 16, 64).as_strided((1, 2, 16, 64), (7, 1024, 64, 1))
     assert attend(k=c[:1], v=one).shape == (1, 2, 64)

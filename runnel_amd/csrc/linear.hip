@@ -329,6 +329,13 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double v) {  // 0 where there is none
+  return __hiloint2double(
+      __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false),
+      __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false));
+}
+
 // Everything of a chunk that no state goes into, a workgroup per (chunk,
 // value head), 16 tokens a wave.  Bound by the latency of its steps, so it
 // keeps few registers and 30 KB of LDS: five workgroups a compute unit.  Each
@@ -351,8 +358,8 @@ __device__ __forceinline__ void prepare(const LinearArgs& a, int64_t block) {
   const int each = a.v_heads / a.k_heads;
   const int hk = hv / each;
   // the last r whose chunks start at or before c: 64 of them looked at at a
-  // time, one a lane (9 sequences of 5 to 1500
-  // tokens: prepared in 12.7 us, 13.1 by bisection)
+  // time, one a lane (9 sequences of 5 to 1500 tokens: prepared in 12.7 us,
+  // 13.1 by bisection)
   int r = 0;
   for (int left = a.requests; left > 1;) {
     const int step = (left + kWave - 1) / kWave;
@@ -389,12 +396,14 @@ __device__ __forceinline__ void prepare(const LinearArgs& a, int64_t block) {
   double G = lane < len ? (double)log_decay(a, row0 + lane, hv) * kLog2e : 0.0;
   float beta = 0.0f;
   if (DELTA && lane < len) beta = a.beta[(row0 + lane) * a.beta_row + hv * a.beta_head];
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const double up = __shfl_up(G, d, kWave);
-    if (lane >= d) G += up;
-  }
-  const double Gc = __shfl(G, 63, kWave);
+  G += from_lane<0x111, 0xf>(G);  // one lane to the left in a row of 16, then 2, 4, 8
+  G += from_lane<0x112, 0xf>(G);
+  G += from_lane<0x114, 0xf>(G);
+  G += from_lane<0x118, 0xf>(G);
+  G += from_lane<0x142, 0xa>(G);  // a row's last lane to the next row, of 32 to the next 32
+  G += from_lane<0x143, 0xc>(G);
+  const double Gc = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(G), kWave - 1),
+                                     __builtin_amdgcn_readlane(__double2loint(G), kWave - 1));
   uint8_t* ws = static_cast<uint8_t*>(a.workspace) +
                 (c * a.v_heads + hv) * (int64_t)ChunkData<DELTA>::bytes;
   if (wave == 0) {

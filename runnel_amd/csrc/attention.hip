@@ -169,6 +169,24 @@ __device__ __forceinline__ T running_sum(T v) {
   return v;
 }
 
+// The greatest of all lanes.
+__device__ __forceinline__ float wave_max(float v) {
+  auto with = [&](auto ctrl, auto rows) {
+    const int w = (int)__float_as_uint(v);  // its own where there is no other
+    v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+                     w, w, decltype(ctrl)::value, decltype(rows)::value, 0xf, false)));
+  };
+  constexpr std::integral_constant<int, 0xf> all;
+  with(std::integral_constant<int, 0x111>(), all);
+  with(std::integral_constant<int, 0x112>(), all);
+  with(std::integral_constant<int, 0x114>(), all);
+  with(std::integral_constant<int, 0x118>(), all);
+  with(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+  with(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+  return __uint_as_float(
+      (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), kWave - 1));
+}
+
 // Part w of all.  Every wave works it out from the lengths (a load and two
 // running sums across the wave for each 64 requests): the parts of all
 // requests are of about one size, total / a.parts, and there is none without
@@ -540,23 +558,30 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   if (parts == 1) return;  // written in the first launch
   const int64_t first = (int64_t)list.x * heads + row % heads;
   const int tid = threadIdx.x, c = tid % C, q = tid / C;
-  float top = -INFINITY;
   const float2* ml = a.part_ml + first;
+  const float* o = a.part_o + first * D + slice * SLICE;
+  auto load = [&](int i) {
+    return reinterpret_cast<const float4*>(o + (int64_t)i * heads * D)[c];
+  };
+  // a thread's first part is on its way while the maximum is found
+  const bool mine = q < Q && q < parts;
+  float2 e = make_float2(-INFINITY, 0.0f);
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (mine) e = ml[(int64_t)q * heads], v = load(q);
+  float top = -INFINITY;
   for (int i = tid & 63; i < parts; i += 64) top = fmaxf(top, ml[(int64_t)i * heads].x);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
+  top = wave_max(top);
   const float base = top == -INFINITY ? 0.0f : top;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float sum = 0.0f;
-#pragma unroll 4
-  for (int i = q; i < (q < Q ? parts : 0); i += Q) {
-    const float2 e = ml[(int64_t)i * heads];
+  auto add = [&](const float2 e, const float4 v) {
     const float f = __builtin_amdgcn_exp2f(e.x - base);
-    const float* part = a.part_o + (first + (int64_t)i * heads) * D + slice * SLICE;
-    const float4 v = reinterpret_cast<const float4*>(part)[c];
     sum += f * e.y;
     acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-  }
+  };
+  if (mine) add(e, v);
+#pragma unroll 4
+  for (int i = q + Q; i < (q < Q ? parts : 0); i += Q) add(ml[(int64_t)i * heads], load(i));
   if (q < Q) {
     acc_s[q][c] = acc;
     if (c == 0) sum_s[q] = sum;

@@ -114,6 +114,7 @@ template <int D>
 struct Runs {
   static constexpr int first = D >= 128 ? 128 : 64;
   static constexpr int second = D - first;
+  static constexpr int row = first + 4;  // of LDS, where heads' rows then lie on other banks
 };
 
 // A request's keys [start, end) and the tiles of 32 they touch.
@@ -252,7 +253,7 @@ void attention_kernel(const AttentionArgs a) {
   constexpr int E0 = P0 / 16, E1 = P1 / 16;
   constexpr int V0 = (E0 * EB + 3) / 4, V1 = (E1 * EB + 3) / 4;  // dwords of a key's runs
   constexpr int KW = KS * 8 * EB / 4;                            // dwords of a key's share
-  extern __shared__ float lds[];
+  extern __shared__ __align__(16) float lds[];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -475,64 +476,88 @@ void attention_kernel(const AttentionArgs a) {
     if (next < t_end) load_v(next, pv);
   }
 
-  // the waves' parts together, a run of dims and four waves at a time
+  // The waves' parts together: first their maxima, so that each wave scales
+  // what it has, then the sums of a run of dims and four waves at a time.
+  // (Instruction fetch counts here: the code runs once.  With every sum's
+  // factors at the sum, a value at a time, this took 7300 of a short part's
+  // 16400 cycles.)
   l = head_sum(l);
   constexpr int THREADS = WAVES * kWave;
-  constexpr int ITEMS = (16 * P0 + THREADS - 1) / THREADS;  // of a thread: (head, dim) pairs
-  float* ml = lds + 4 * heads * P0;  // [wave][head] maximum, then sum
+  constexpr int ROW = Runs<D>::row;
+  constexpr int ITEMS = (16 * P0 / 4 + THREADS - 1) / THREADS;  // of a thread: four dims of a head
+  float* ml = lds + 4 * heads * ROW;  // [wave][head] maximum, then sum, then both of all
   if (n < heads && g == 0) {
     ml[wave * 16 + n] = m;
     ml[(WAVES + wave) * 16 + n] = l;
+  }
+  __syncthreads();
+  float* of_all = ml + 2 * WAVES * 16;
+  if (n < heads) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml[w * 16 + n]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      sum += __builtin_amdgcn_exp2f(ml[w * 16 + n] - base) * ml[(WAVES + w) * 16 + n];
+    const float f = __builtin_amdgcn_exp2f(m - base);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i] *= f;
+    if (wave == 0 && g == 0) of_all[n] = top, of_all[16 + n] = sum;
   }
   const int64_t row = (int64_t)r * a.kv_heads * a.group + head0;
   auto join = [&](auto run) {
     constexpr int P = decltype(run)::value ? P1 : P0, E = P / 16;
     constexpr int I0 = decltype(run)::value ? E0 : 0, D0 = decltype(run)::value ? P0 : 0;
-    float acc[ITEMS], sum[ITEMS], top[ITEMS];
+    f32x4 acc[ITEMS];
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) acc[q] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w0 = 0; w0 < WAVES; w0 += 4) {
       if (w0 || D0) __syncthreads();
       if (n < heads && wave >= w0 && wave < w0 + 4) {
-        float* mine = lds + ((wave - w0) * heads + n) * P + 4 * g * E;
+        float* mine = lds + ((wave - w0) * heads + n) * ROW + 4 * g * E;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (E >= 4) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mine[k * E + i] = o[I0 + i][k];
+            for (int i = 0; i < E; i += 4)
+              *reinterpret_cast<f32x4*>(mine + k * E + i) =
+                  (f32x4){o[I0 + i][k], o[I0 + i + 1][k], o[I0 + i + 2][k], o[I0 + i + 3][k]};
+          } else {
+            static_assert(E >= 4 || E == 2 || E == 0, "runs of 128, 64 or 32");
+            *reinterpret_cast<f32x2*>(mine + k * E) = (f32x2){o[I0][k], o[I0 + 1][k]};
+          }
+        }
       }
       __syncthreads();
 #pragma unroll
       for (int q = 0; q < ITEMS; ++q) {
-        const int i = tid + q * THREADS;
-        if (i >= heads * P) continue;
-        const int h = i / P, d = i - h * P;
-        if (w0 == 0) {
-          acc[q] = sum[q] = 0.0f, top[q] = -INFINITY;
+        const int i = tid + q * THREADS, h = i / (P / 4), d = i % (P / 4) * 4;
+        if (h >= heads) continue;
 #pragma unroll
-          for (int w = 0; w < WAVES; ++w) top[q] = fmaxf(top[q], ml[w * 16 + h]);
-        }
-        const float base = top[q] == -INFINITY ? 0.0f : top[q];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float f = __builtin_amdgcn_exp2f(ml[(w0 + w) * 16 + h] - base);
-          sum[q] += f * ml[(WAVES + w0 + w) * 16 + h];
-          acc[q] += f * lds[(w * heads + h) * P + d];
-        }
+        for (int w = 0; w < 4; ++w)
+          acc[q] += *reinterpret_cast<const f32x4*>(lds + (w * heads + h) * ROW + d);
       }
     }
 #pragma unroll
     for (int q = 0; q < ITEMS; ++q) {
-      const int i = tid + q * THREADS;
-      if (i >= heads * P) continue;
-      const int h = i / P, d = D0 + i - h * P;
+      const int i = tid + q * THREADS, h = i / (P / 4), d = D0 + i % (P / 4) * 4;
+      if (h >= heads) continue;
+      const float top = of_all[h], sum = of_all[16 + h];
       if (parts == 1) {
-        const bool some = sum[q] > 0.0f || sum[q] != sum[q];
-        a.out[(row + h) * D + d] = (uint16_t)f32_to_bf16(some ? acc[q] / sum[q] * a.v_scale : 0.0f);
-        if (a.lse && d == 0)
-          a.lse[row + h] = top[q] == -INFINITY ? top[q] : (top[q] + log2f(sum[q])) * kLn2;
+        const bool some = sum > 0.0f || sum != sum;
+        uint32_t x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k] = f32_to_bf16(some ? acc[q][k] / sum * a.v_scale : 0.0f);
+        *reinterpret_cast<uint2*>(a.out + (row + h) * D + d) =
+            make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
+        if (a.lse && d == 0) a.lse[row + h] = top == -INFINITY ? top : (top + log2f(sum)) * kLn2;
       } else {
         const int64_t at = (int64_t)w * a.kv_heads * a.group + head0 + h;
-        a.part_o[at * D + d] = acc[q];
-        if (d == 0) a.part_ml[at] = make_float2(top[q], sum[q]);
+        *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = acc[q];
+        if (d == 0) a.part_ml[at] = make_float2(top, sum);
       }
     }
   };
@@ -614,7 +639,7 @@ hipError_t launch_attention_of(const AttentionArgs& a, hipStream_t s) {
   const int64_t parts = a.all_parts >= 8 ? (a.all_parts + 7) / 8 * 8 : a.all_parts;
   const unsigned grid = (unsigned)(parts * a.kv_heads * a.head_tiles);
   auto lds = [&](int waves) {
-    return (size_t)(4 * heads * Runs<D>::first + 2 * waves * 16) * sizeof(float);
+    return (size_t)(4 * heads * Runs<D>::row + 2 * (waves + 1) * 16) * sizeof(float);
   };
   if (a.alone) {
     attention_kernel<D, E4M3, kAloneWaves>

@@ -666,9 +666,9 @@ hipError_t launch_attention_dim(const AttentionArgs& a, hipStream_t s) {
 
 // Up to this many values of K a request that would be split is left whole to
 // one workgroup of eight waves, without a second launch (one request, 2 key
-// heads of 128 dims: 130 keys 8.6 us against 9.7, 500 keys 10.9 against 10.6
-// and a launch less on the host; 1000 keys 15.5 against 10.7: one compute unit
-// reads 60 GB/s).
+// heads of 128 dims: 130 keys 6.4 us against 8.5, 500 keys 9.6 against 8.8 and
+// a launch, 3 us, less on the host; 1000 keys 14.0 against 8.8: one compute
+// unit reads 60 GB/s).
 constexpr int64_t kAloneValues = 512 * 128;
 
 AttentionPlan attention_plan(int requests, int kv_heads, int group, int dim, int64_t keys) {
@@ -685,14 +685,19 @@ AttentionPlan attention_plan(int requests, int kv_heads, int group, int dim, int
     return each > 1 ? AttentionPlan{(int)(each * requests), (int)(each * requests), 0} : whole;
   }
   // Workgroups: of wide heads, whose registers leave room for one or two a
-  // compute unit, one each (4 requests of 1000 to 40000 keys, 2 heads of 256:
-  // 31 us, 40 with 512, 60 with 1024); of others two for a single request
-  // (131071 keys, 8 heads of 128, 8 bits: 57 us, 63 with 1536), and six where
-  // requests differ (61 of 17 to 16000 keys, 8 heads: 72 us, 83 with 512, 75
-  // with 4096).  Where that is less than a part a request, the parts are of
-  // the average request's size (256 of 700 to 4100 keys, 16 heads of 64: 367
-  // us, with larger ones 392).
-  int64_t parts = (dim > 128 ? 256 : requests == 1 ? 512 : 1536) / heads;
+  // compute unit, whole rounds of one each with the rounding of every request's
+  // parts counted in, the fewest in which a part is no more than the average
+  // request (20 requests of 1000 to 30000 keys, 2 heads of 256: 76 us, 97 if
+  // the rounding starts a second round; 4 of 1000 to 40000 28, 32 with two
+  // rounds); of others two each for a single request (131071 keys, 8 heads of
+  // 128, 8 bits: 57 us, 63 with six), and six where requests differ (61 of 17
+  // to 16000 keys, 8 heads: 72 us, 83 with two, 75 with sixteen).  Where that
+  // is less than a part a request, the parts are of the average request's size
+  // (256 of 700 to 4100 keys, 16 heads of 64: 367 us, with larger ones 392).
+  const int64_t units = 256 / heads;
+  int64_t parts = requests == 1 ? (dim > 128 ? units : 512 / heads) : 1536 / heads;
+  if (dim > 128 && requests > 1 && units > 0)
+    parts = (2 * requests + units - 1) / units * units - requests;
   if (parts < requests) parts = requests;
   const int64_t most = (tiles + kAttWaves - 1) / kAttWaves * requests;
   if (parts > most) parts = most;

@@ -471,6 +471,14 @@ def test_attention_ragged(native, R, bits):
         check_attention(native, q, kc, vc, table, some)
 
 
+@pytest.mark.parametrize("R,hk,D", [(2, 1, 256), (21, 2, 256), (40, 3, 192)])
+def test_attention_ragged_wide(native, R, hk, D):
+    """Wide heads, whose parts are counted in whole rounds of workgroups."""
+    lens = [(40, 1, 0, 150, 65)[i % 5] for i in range(R)]
+    lens[1] = 1200
+    check_attention(native, *attention_inputs(D + R, lens, 2 * hk, hk, D, 16, 16 if R < 40 else 8))
+
+
 @pytest.mark.parametrize("hq,hk", [(40, 2), (6, 6)])
 def test_attention_ragged_heads(native, hq, hk):
     """Several heads of keys, and more than a tile of query heads to one."""

@@ -881,6 +881,30 @@ def test_streams_share_nothing(native):
                 assert torch.equal(x, y)
 
 
+def test_threads(native):
+    """Calls from several Python threads, each on a stream of its own: the
+    binding lets others run while it launches, and errors stay with theirs."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    q, kc, vc, table, lengths = attention_inputs(2, [1500, 40, 7], 4, 2, 64, 16, 16)
+    a = [q.cuda(), kc, vc, table.cuda(), lengths.cuda()]
+    b = [None if y is None else y.cuda() for y in linear_inputs(2, [90, 3], 2, 4, 64, 32)]
+    want = native.paged_attention(*a), native.linear_attention(*b[:5], b[5].clone(), beta=b[6])
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                assert torch.equal(native.paged_attention(*a), want[0])
+                assert torch.equal(native.linear_attention(*b[:5], b[5].clone(), beta=b[6]), want[1])
+                with pytest.raises(ValueError, match="page_size" if i % 2 else "rows must not"):
+                    native.paged_tables(a[4], a[4], a[3].clone(), a[4], 12 if i % 2 else 16, 1 if i % 2 else -1)
+        return i
+
+    with ThreadPoolExecutor(4) as pool:
+        assert list(pool.map(work, range(4))) == [0, 1, 2, 3]
+
+
 def test_two_graphs(native):
     """Two captured graphs of the same operators, replayed in turn and at
     once on two streams."""
